@@ -19,9 +19,14 @@ FERRET_SILU_MUL = 0x1
 FERRET_TILE_SHIFT = 8
 FERRET_UE8M0_SCALES = 0x2
 FERRET_PREFILL_PAIRS = 0x4
+FERRET_BF16, FERRET_FP16, FERRET_FP32 = 0, 1, 2
+FERRET_ROUTE_SIGMOID = 0x1
+FERRET_ROUTE_RENORM = 0x2
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
+_l = ctypes.c_longlong
+_f = ctypes.c_float
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/ferret_moe.h
@@ -52,6 +57,17 @@ SIGNATURES = {
     "ferret_fp8_grouped_gemm_nt_contiguous_noalloc": (
         _i, [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p]),
     "ferret_moe_combine": (_i, [_p, _p, _p, _i, _i, _i, _i, _p, _p]),
+    "ferret_add_rms_norm": (
+        _i, [_p, _l, _p, _l, _p, _i, _i, _i, _i, _f, _p, _p, _p, _p, _i, _p]),
+    "ferret_moe_route": (
+        _i, [_p, _l, _i, _p, _p, _i, _i, _i, _i, _i, _i, _f, _i, _p, _p, _p]),
+    "ferret_moe_route_backward": (_i, [_p, _p, _l, _i, _p, _i, _i, _i, _f, _i, _p, _p]),
+    "ferret_moe_balance_loss_workspace_size": (_sz, [_i, _i]),
+    "ferret_moe_balance_loss": (
+        _i, [_p, _l, _i, _p, _p, _i, _i, _i, _f, _i, _p, _p, _p, _p, _p, _sz, _p]),
+    "ferret_moe_balance_loss_backward": (
+        _i, [_p, _p, _l, _i, _p, _p, _p, _i, _i, _i, _f, _i, _p, _p]),
+    "ferret_int4_linear": (_i, [_p, _l, _p, _p, _p, _p, _i, _i, _i, _i, _i, _p, _p]),
     "ferret_ep_handle_bytes": (_sz, []),
     "ferret_ep_init": (_i, [_i, _i, _i, _i, _i, _i, _i, _i, _p, _p, ctypes.POINTER(_p)]),
     "ferret_ep_connect": (_i, [_p, _p]),

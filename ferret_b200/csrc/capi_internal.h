@@ -126,11 +126,11 @@ inline bool kernel_has_regs(void (*kern)(KArgs...), int regs) {
     return fa.numRegs >= regs;
 }
 
-// The same for a kernel of CTA pairs (thread-block clusters of 2 along x).
-// grid.x must be even.
+// The same for a kernel of thread-block clusters of `cluster` CTAs along x.
+// grid.x must be a multiple of it.
 template <typename... KArgs, typename... Args>
-inline int launch_kernel_pairs(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                               cudaStream_t stream, Args&&... args) {
+inline int launch_kernel_cluster(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                 int cluster, cudaStream_t stream, Args&&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -140,7 +140,7 @@ inline int launch_kernel_pairs(void (*kern)(KArgs...), dim3 grid, dim3 block, si
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
@@ -150,6 +150,14 @@ inline int launch_kernel_pairs(void (*kern)(KArgs...), dim3 grid, dim3 block, si
         return FERRET_ERR_CUDA;
     }
     return FERRET_OK;
+}
+
+// The same for a kernel of CTA pairs (thread-block clusters of 2 along x).
+// grid.x must be even.
+template <typename... KArgs, typename... Args>
+inline int launch_kernel_pairs(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                               cudaStream_t stream, Args&&... args) {
+    return launch_kernel_cluster(kern, grid, block, smem, 2, stream, std::forward<Args>(args)...);
 }
 
 // How many CTA pairs of `kern` (block threads, smem bytes) can be resident at

@@ -13,6 +13,7 @@
 //
 // HBM-bound: a warp quantizes 4 blocks of a row per task, 16 bytes per lane in.
 #include "capi_internal.h"
+#include "fp8_quant.cuh"
 
 namespace ferret {
 namespace {
@@ -27,8 +28,6 @@ __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w 
 // covers one block with 16-byte loads; both loads of a lane are issued before
 // either is used, so 1 KB per warp is in flight (the kernel is bound by the
 // latency of the gathered row reads, not by HBM, at decode sizes).
-// UE8M0: the scale is the smallest power of two >= fl(amax / 448), taken from
-// the fp32 bits (exact; no log2), and x is multiplied by its exact inverse.
 // SCATTER: row r is token r (R = x_rows), and its quantized row is written to
 // every row inv[r * gather_div + j], j < gather_div, that is not negative (the
 // expert-sorted positions of the token's top-k pairs): each token is
@@ -83,45 +82,21 @@ __global__ void __launch_bounds__(kQuantThreads)
             for (int off = 8; off > 0; off >>= 1)      // within the 16-lane half
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
             if (b >= nk) continue;
-            amax = fmaxf(amax, 1e-4f);
-            float f, sc;
-            if (UE8M0) {
-                const uint32_t bits = __float_as_uint(__fdiv_rn(amax, 448.0f));
-                const uint32_t ex = (bits >> 23) + ((bits & 0x7FFFFFu) ? 1u : 0u);
-                sc = __uint_as_float(ex >= 255u ? 0x7F800000u : ex << 23);
-                f = ex >= 255u ? 0.0f
-                               : __uint_as_float(ex == 254u ? 0x00400000u : (254u - ex) << 23);
-            } else {
-                // `448.0 / amax` in the published torch code is reciprocal-then-multiply
-                f = __fmul_rn(__frcp_rn(amax), 448.0f);
-                sc = __fdiv_rn(amax, 448.0f);
-            }
-            uint32_t packed[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(
-                    make_float2(__fmul_rn(v[4 * j], f), __fmul_rn(v[4 * j + 1], f)), __NV_SATFINITE,
-                    __NV_E4M3);
-                const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(
-                    make_float2(__fmul_rn(v[4 * j + 2], f), __fmul_rn(v[4 * j + 3], f)),
-                    __NV_SATFINITE, __NV_E4M3);
-                packed[j] = (uint32_t)lo | ((uint32_t)hi << 16);
-            }
+            const Fp8Scale fs = fp8_block_scale(amax, UE8M0);
+            const float sc = fs.scale;
+            uint2 packed = fp8_pack8(v, fs.mul);
             if (SCATTER) {
                 for (int j = 0; j < gather_div; ++j) {
                     const int p = __ldg(gather + (long long)r * gather_div + j);
                     if (p < 0) continue;
-                    *reinterpret_cast<uint2*>(q + (long long)p * K + b * 128 + hl * 8) =
-                        make_uint2(packed[0], packed[1]);
+                    *reinterpret_cast<uint2*>(q + (long long)p * K + b * 128 + hl * 8) = packed;
                     if (hl == 0) scale[(long long)p * nk + b] = sc;
                 }
                 continue;
             }
             uint8_t* qdst = q + (long long)r * K + b * 128 + hl * 8;
-            if (src < 0) {
-                packed[0] = packed[1] = 0u;
-            }
-            *reinterpret_cast<uint2*>(qdst) = make_uint2(packed[0], packed[1]);
+            if (src < 0) packed = make_uint2(0u, 0u);
+            *reinterpret_cast<uint2*>(qdst) = packed;
             if (hl == 0) scale[(long long)r * nk + b] = src < 0 ? 0.0f : sc;
         }
     }

@@ -60,6 +60,16 @@ extern "C" {
                                        block-scaled pair kernel on whole 256-row chunks, the rest
                                        on single CTAs); same results, measured slower */
 
+
+/* element types of the entry points that take one (`dtype`) */
+#define FERRET_BF16 0
+#define FERRET_FP16 1
+#define FERRET_FP32 2
+
+/* flags of the routing and balance-loss entry points */
+#define FERRET_ROUTE_SIGMOID 0x1    /* scores are sigmoids (default: softmax over the experts) */
+#define FERRET_ROUTE_RENORM 0x2     /* a token's weights are divided by their sum */
+
 /* Library version (FERRET_MOE_VERSION). */
 FERRET_API int ferret_version(void);
 
@@ -322,6 +332,124 @@ FERRET_API int ferret_int4_moe_w13(const void* hidden_bf16, const void* w_blob,
                                    const int32_t* sorted_rows, const int32_t* expert_offsets,
                                    void* out_bf16, int T, int topk, int N, int K, int E, int flags,
                                    void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Residual addition, RMS norm and 1x128 FP8 rows in one pass (no reference
+ * counterpart: the step in front of the expert layer, whose FP8 rows the
+ * grouped GEMM reads).  Per row of K columns:
+ *   s = x + residual (fp32; s = x without a residual), residual_out = round(s)
+ *   y = s * (mean(s^2) + eps)^(-1/2) * weight, stored rounded to `dtype`
+ *   q_fp8 / q_scale: y quantized as ferret_quant_act_fp8_1x128 does (as
+ *   ferret_quant_act_fp8_1x128_ue8m0 with flags = FERRET_UE8M0_SCALES), from
+ *   the fp32 y, not from the stored one.
+ * x, residual: `dtype` [T, K], row strides ldx, ldr in elements (ldr is not
+ * read without a residual); weight [K] of weight_dtype (`dtype` or
+ * FERRET_FP32).  Outputs are contiguous; y or q_fp8 may be NULL (not both),
+ * residual_out too; q_scale is [T, K/128].  residual_out may be the same
+ * memory as x or residual when that one is contiguous; any other overlap of
+ * inputs and outputs is undefined.
+ * Limits: K <= 32768; K % 128 == 0 with q_fp8; eps >= 0.  Rows that do not all
+ * start on a 16-byte boundary take element-wise loads (same result).
+ */
+FERRET_API int ferret_add_rms_norm(const void* x, long long ldx, const void* residual,
+                                   long long ldr, const void* weight, int weight_dtype, int dtype,
+                                   int T, int K, float eps, void* y, void* residual_out,
+                                   void* q_fp8, float* q_scale, int flags, void* stream);
+
+/*
+ * Router: the top-k ids and weights of every token from its expert logits
+ * (no reference counterpart: the reference draws synthetic ids,
+ * baselines/kimi-moe-w13-int4/baseline_marlin.py:92-104; their layout is the
+ * one ferret_moe_permute and ferret_moe_combine read).
+ * logits: `dtype` [T, E], row stride ld in elements.
+ * score = softmax over the E logits, or sigmoid (FERRET_ROUTE_SIGMOID);
+ * key = score + bias[e] (bias f32 [E] or NULL).  With n_group > 1 the experts
+ * form n_group equal consecutive groups, a group's score is the sum of its
+ * group_top (1 or 2) largest keys, and experts outside the topk_group best
+ * groups are closed.  The topk largest keys win, in descending order; equal
+ * keys (and equal groups) go to the lower index.  The order is that of the
+ * exact keys: keys closer than their fp32 rounding are compared in fp64.
+ * ids int32 [T, topk]; weights f32 [T, topk] = scale * score (without the
+ * bias), divided by the sum of the token's chosen scores with
+ * FERRET_ROUTE_RENORM (0 if that sum is 0).
+ * A logit of -inf or NaN, or a bias of -inf or NaN, closes its expert; +inf
+ * counts as the largest finite value.  Slots without an open expert, and all
+ * slots of a token whose token_mask byte (uint8 [T] or NULL) is 0, have id -1
+ * and weight 0.
+ * Limits: E <= 1024, topk <= 32, topk <= topk_group * E / n_group, n_group a
+ * power of two up to 32 that divides E.
+ */
+FERRET_API int ferret_moe_route(const void* logits, long long ld, int dtype, const float* bias,
+                                const uint8_t* token_mask, int T, int E, int topk, int n_group,
+                                int topk_group, int group_top, float scale, int flags,
+                                float* weights, int32_t* ids, void* stream);
+
+/*
+ * Gradient of the logits from the gradient of ferret_moe_route's weights (ids,
+ * scale and flags as there; the choice itself has no gradient).
+ * grad_weights f32 [T, topk]; grad_logits: `dtype` [T, E] contiguous, written
+ * in full (zero where a logit does not enter).  Slots whose id is outside
+ * [0, E) count for nothing; slots that repeat an id add up.
+ */
+FERRET_API int ferret_moe_route_backward(const float* grad_weights, const void* logits,
+                                         long long ld, int dtype, const int32_t* ids, int T, int E,
+                                         int topk, float scale, int flags, void* grad_logits,
+                                         void* stream);
+
+/*
+ * Balance loss of a routed batch, with the per-expert counts (no reference
+ * counterpart).  Over the V tokens whose token_mask byte is not 0 (NULL: all):
+ *   counts[e] = number of (token, slot) pairs with topk_ids == e (ids outside
+ *               [0, E) count for nothing)
+ *   prob_sums[e] = sum over the tokens of p[t, e], p = softmax(logits) or, with
+ *               FERRET_ROUTE_SIGMOID, sigmoids divided by their sum over e
+ *   n_tokens = V
+ *   loss = coef * E / (topk * V^2) * sum_e counts[e] * prob_sums[e]  (0 if V == 0)
+ * logits of -inf or NaN have p = 0.  logits `dtype` [T, E] with row stride ld,
+ * topk_ids int32 [T, topk]; loss, n_tokens one element each.
+ * The sums have a fixed order: same inputs on the same device, same bits.
+ * workspace: ferret_moe_balance_loss_workspace_size(T, E) bytes, 4-byte
+ * aligned, not shared by calls that can run at the same time.
+ * Limits: E <= 1024.
+ */
+FERRET_API size_t ferret_moe_balance_loss_workspace_size(int T, int E);
+FERRET_API int ferret_moe_balance_loss(const void* logits, long long ld, int dtype,
+                                       const int32_t* topk_ids, const uint8_t* token_mask, int T,
+                                       int E, int topk, float coef, int flags, float* loss,
+                                       int32_t* counts, float* prob_sums, int32_t* n_tokens,
+                                       void* workspace, size_t ws_bytes, void* stream);
+
+/*
+ * Gradient of the logits from grad_loss (f32, one element, device memory);
+ * counts and n_tokens as ferret_moe_balance_loss wrote them (or summed over
+ * data-parallel ranks), constants of the gradient.  grad_logits: `dtype`
+ * [T, E] contiguous, written in full; masked tokens get zero rows.
+ */
+FERRET_API int ferret_moe_balance_loss_backward(const float* grad_loss, const void* logits,
+                                                long long ld, int dtype, const int32_t* counts,
+                                                const int32_t* n_tokens, const uint8_t* token_mask,
+                                                int T, int E, int topk, float coef, int flags,
+                                                void* grad_logits, void* stream);
+
+/*
+ * Few tokens times one dense 4-bit weight matrix (the dense counterpart of
+ * ferret_int4_moe_w13: shared experts and projections of an INT4 checkpoint).
+ *   y[t, n] = sum_k x[t, k] * scale[k/g, n] * (nibble(k, n) - zero[k/g, n]) + bias[n]
+ * x `dtype` (FERRET_BF16 or FERRET_FP16) [T, K] with row stride ldx; w int32
+ * [K/8, N], the raw compressed-tensors layout of ferret_int4_repack_w13 (eight
+ * nibbles along K per word, low nibble first), read as it is; w_scale `dtype`
+ * [K/group, N]; w_zero NULL (zero = 8) or int32 [K/group, N/8], eight nibbles
+ * along N per word, low nibble first; bias NULL or `dtype` [N]; y `dtype`
+ * [T, N] contiguous.  fp32 sums, scales applied in fp32, one rounding at the
+ * end; the order of the sums is fixed.  Each pass over the weights serves up
+ * to 32 tokens, so more tokens read them again.
+ * Limits: group % 32 == 0, K % group == 0, N % 8 == 0, ldx % 8 == 0; x and w
+ * 16-byte aligned, w_scale 8-byte.
+ */
+FERRET_API int ferret_int4_linear(const void* x, long long ldx, const int32_t* w,
+                                  const void* w_scale, const int32_t* w_zero, const void* bias,
+                                  int dtype, int T, int K, int N, int group, void* y,
+                                  void* stream);
 
 /*
  * Expert-parallel FP8 W13 over NVLink peer memory, one process per GPU.

@@ -15,22 +15,27 @@
 // -inf or NaN have p = 0.
 //
 // HBM-bound: forward reads the logits once; backward reads them once and writes
-// the gradient once.  A warp takes a token at a time with its row in registers
-// and sums probabilities for its 32 x VPL columns in registers over all its
+// the gradient once.  LPT lanes share a token's row, NV vectors of 4 columns
+// each, and the next token's row is loaded before the current one is used.  The
+// forward kernel sums probabilities for its columns in registers over all its
 // tokens, so the only reduction across CTAs is one [CTAs, E] table of partial
-// sums and counts in the workspace.  A second launch adds its rows in CTA
-// order: no floating-point atomics, the same bits every time.
+// sums and counts in the workspace.  A second launch (128 columns per CTA, one
+// cluster) adds its rows in a fixed order: no floating-point atomics, the same
+// bits every time.
 #include <algorithm>
+#include <cooperative_groups.h>
 
 #include "row_io.cuh"
 
 namespace ferret {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kBalWarps = 8;
 constexpr int kBalThreads = kBalWarps * 32;
 constexpr int kBalMaxE = 1024;
-constexpr int kBalTokensPerWarp = 2;   // below this many a further CTA costs more than it saves
+constexpr int kBalMaxCtas = 256 * 4;   // partial rows, on the largest device
 
 struct BalanceArgs {
     const void* logits;
@@ -44,82 +49,126 @@ struct BalanceArgs {
     int32_t* part_live;   // [ctas]
 };
 
-// A token's probabilities in registers, column 32 k + lane (all zero for a row
-// of closed logits), and the factor of the gradient that the scoring adds:
-// 1 - sigmoid(z), or 1 for the softmax.
-template <typename LT, int VPL>
-__device__ __forceinline__ void row_probs(const LT* row, int E, bool sigmoid, float (&p)[VPL],
-                                          float (&rest)[VPL]) {
-    const int lane = threadIdx.x & 31;
-    float m = -INFINITY;
+// A row's pieces as loaded: vector i of a lane holds columns 4 (LPT i + lane) ..+3.
+template <typename LT, int NV>
+struct RowRaw {
+    LT e[NV][4];
+};
+
+template <typename LT, int LPT, int NV, bool VEC>
+__device__ __forceinline__ RowRaw<LT, NV> load_row(const LT* row, int E) {
+    RowRaw<LT, NV> r;
+    const int sub = threadIdx.x % LPT;
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        const int e = 32 * k + lane;
-        const float z = e < E ? to_f32(row[e]) : -INFINITY;
-        p[k] = z > -INFINITY ? fminf(z, 3.402823466e38f) : -INFINITY;
-        m = fmaxf(m, p[k]);
-    }
-    float sum = 0.0f;
-    if (sigmoid) {
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            const float e = expf(-fabsf(p[k])), r = 1.0f / (1.0f + e);
-            rest[k] = p[k] >= 0.0f ? e * r : r;
-            p[k] = p[k] >= 0.0f ? r : e * r;      // -inf: e = 0
-            sum += p[k];
-        }
-    } else {
-        m = warp_max(m);
-        const float shift = m > -INFINITY ? m : 0.0f;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) {
-            p[k] = expf(p[k] - shift);
-            rest[k] = 1.0f;
-            sum += p[k];
-        }
-    }
-    sum = warp_sum(sum);
-    if (sum < 0x1p-100f) {                        // sigmoids of far negative logits alone
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) p[k] *= 0x1p100f;
-        sum *= 0x1p100f;
-    }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int k = 0; k < VPL; ++k) p[k] *= inv;
+    for (int i = 0; i < NV; ++i) load4<LT, VEC>(row, 4 * (LPT * i + sub), E, r.e[i]);
+    return r;
 }
 
-template <typename LT, int VPL>
+// Its probabilities (all zero for a row of closed logits), and the factor that
+// the scoring adds to the gradient: 1 - sigmoid(z), or 1 for the softmax.
+template <typename LT, int LPT, int NV>
+__device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool sigmoid,
+                                          float (&p)[NV][4], float (&rest)[NV][4]) {
+    const int sub = threadIdx.x % LPT;
+    float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float z = clean_logit(to_f32(r.e[i][k]));
+            p[i][k] = 4 * (LPT * i + sub) + k < E ? z : -INFINITY;
+            m = fmaxf(m, p[i][k]);
+        }
+    if (sigmoid) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float z = p[i][k], e = expf(-fabsf(z)), inv = 1.0f / (1.0f + e);
+                rest[i][k] = z >= 0.0f ? e * inv : inv;
+                p[i][k] = z >= 0.0f ? inv : e * inv;      // -inf: e = 0
+                sum += p[i][k];
+            }
+    } else {
+        m = lanes_max<LPT>(m);
+        const float shift = m > -INFINITY ? m : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                p[i][k] = expf(p[i][k] - shift);
+                rest[i][k] = 1.0f;
+                sum += p[i][k];
+            }
+    }
+    sum = lanes_sum<LPT>(sum);
+    float scale = 1.0f;
+    if (sum < 0x1p-100f) scale = 0x1p100f;        // sigmoids of far negative logits alone
+    sum *= scale;
+    scale = sum > 0.0f ? scale / sum : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) p[i][k] *= scale;
+}
+
+template <typename LT, int LPT, int NV, bool VEC>
 __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceArgs a) {
     pdl_begin();
-    __shared__ float sums[kBalWarps][32 * VPL];
-    __shared__ int counts[32 * VPL];
+    constexpr int kCols = LPT * NV * 4, kSubs = kBalThreads / LPT;
+    __shared__ float sums[kBalWarps][kCols];
+    __shared__ int counts[kCols];
     __shared__ int live;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e < 32 * VPL; e += kBalThreads) counts[e] = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = threadIdx.x / LPT;
+    // this CTA's tokens, a contiguous run
+    const int t0 = (int)((long long)a.T * blockIdx.x / gridDim.x);
+    const int t1 = (int)((long long)a.T * (blockIdx.x + 1) / gridDim.x);
+    const LT* logits = static_cast<const LT*>(a.logits);
+    auto row_of = [&](int t) { return logits + (long long)min(t, t1 - 1) * a.ld; };
+    RowRaw<LT, NV> next = load_row<LT, LPT, NV, VEC>(row_of(t0 + sub), a.E);
+
+    for (int e = threadIdx.x; e < kCols; e += kBalThreads) counts[e] = 0;
     if (threadIdx.x == 0) live = 0;
     __syncthreads();
+    const long long first = (long long)t0 * a.topk, pairs = (long long)(t1 - t0) * a.topk;
+    for (long long i = threadIdx.x; i < pairs; i += kBalThreads) {
+        const int e = a.ids[first + i];
+        if (e >= 0 && e < a.E && (!a.mask || a.mask[t0 + (int)(i / a.topk)]))
+            atomicAdd(&counts[e], 1);
+    }
 
-    float acc[VPL];
+    float acc[NV][4];
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) acc[k] = 0.0f;
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     int mine = 0;
-    for (long long t = (long long)blockIdx.x * kBalWarps + warp; t < a.T;
-         t += (long long)gridDim.x * kBalWarps) {
-        if (a.mask && !a.mask[t]) continue;
-        ++mine;
-        float p[VPL], rest[VPL];
-        row_probs<LT, VPL>(static_cast<const LT*>(a.logits) + t * a.ld, a.E, a.sigmoid, p, rest);
+    const int rounds = (t1 - t0 + kSubs - 1) / kSubs;
+    for (int n = 0; n < rounds; ++n) {
+        const int t = t0 + n * kSubs + sub;
+        const RowRaw<LT, NV> row = next;
+        if (n + 1 < rounds) next = load_row<LT, LPT, NV, VEC>(row_of(t + kSubs), a.E);
+        const bool counted = t < t1 && (!a.mask || a.mask[t]);
+        mine += counted;
+        float p[NV][4], rest[NV][4];
+        row_probs<LT, LPT, NV>(row, a.E, a.sigmoid, p, rest);
 #pragma unroll
-        for (int k = 0; k < VPL; ++k) acc[k] += p[k];
-        for (int j = lane; j < a.topk; j += 32) {
-            const int e = a.ids[t * a.topk + j];
-            if (e >= 0 && e < a.E) atomicAdd(&counts[e], 1);
-        }
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][k] += counted ? p[i][k] : 0.0f;
     }
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) sums[warp][32 * k + lane] = acc[k];
-    if (lane == 0 && mine) atomicAdd(&live, mine);
+    for (int o = LPT; o < 32; o <<= 1)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[i][k] += __shfl_xor_sync(0xffffffffu, acc[i][k], o);
+    if (lane < LPT)
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sums[warp][4 * (LPT * i + lane) + k] = acc[i][k];
+    if (threadIdx.x % LPT == 0 && mine) atomicAdd(&live, mine);
     __syncthreads();
     for (int e = threadIdx.x; e < a.E; e += kBalThreads) {
         float s = 0.0f;
@@ -131,63 +180,80 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceA
     if (threadIdx.x == 0) a.part_live[blockIdx.x] = live;
 }
 
-// Adds the partial tables' rows in order and forms the loss.  One CTA: its
-// threads split into groups of consecutive experts times slices of the rows.
-__global__ void __launch_bounds__(1024)
-    moe_balance_join_kernel(const float* __restrict__ part_sums,
-                            const int32_t* __restrict__ part_counts,
-                            const int32_t* __restrict__ part_live, int ctas, int E, int topk,
-                            float coef, float* __restrict__ loss, int32_t* __restrict__ counts,
-                            float* __restrict__ prob_sums, int32_t* __restrict__ n_tokens) {
+// Adds the partial tables' rows in a fixed order and forms the loss.  A CTA
+// takes 128 columns, 4 per lane; warp w adds rows w, w + 32, ...
+constexpr int kJoinThreads = 1024;
+constexpr int kJoinCols = 128;
+
+__global__ void __launch_bounds__(kJoinThreads)
+    moe_balance_join_kernel(const float* part_sums, const int32_t* part_counts,
+                            const int32_t* part_live, int ctas, int E, int topk, float coef,
+                            float* loss, int32_t* counts, float* prob_sums, int32_t* n_tokens) {
     pdl_begin();
-    __shared__ float s_sum[1024];
-    __shared__ int s_cnt[1024];
-    __shared__ double s_loss[32];
-    __shared__ int s_live;
-    const int tid = threadIdx.x;
-    const int width = min(1024, (E + 31) / 32 * 32), slices = 1024 / width;
-    const int e = tid % width, slice = tid / width;
-    float s = 0.0f;
-    int c = 0;
-    if (tid == 0) s_live = 0;
-    if (e < E && slice < slices) {
-        const int lo = (int)((long long)ctas * slice / slices),
-                  hi = (int)((long long)ctas * (slice + 1) / slices);
-#pragma unroll 8
-        for (int i = lo; i < hi; ++i) {
-            s += part_sums[(long long)i * E + e];
-            c += part_counts[(long long)i * E + e];
-        }
-    }
-    s_sum[tid] = s;
-    s_cnt[tid] = c;
-    __syncthreads();
-    int v = 0;
-    for (int i = tid; i < ctas; i += 1024) v += part_live[i];
-    if (v) atomicAdd(&s_live, v);
-    double part = 0.0;
-    if (tid < E) {
-        s = 0.0f;
-        c = 0;
-        for (int i = 0; i < slices; ++i) {
-            s += s_sum[i * width + tid];
-            c += s_cnt[i * width + tid];
-        }
-        prob_sums[tid] = s;
-        counts[tid] = c;
-        part = (double)c * (double)s;
-    }
+    __shared__ float s_sum[32][kJoinCols];
+    __shared__ int s_cnt[32][kJoinCols];
+    __shared__ int s_live[32];
+    __shared__ double s_loss[kJoinCols / 32];
+    __shared__ double cta_loss;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int e0 = blockIdx.x * kJoinCols;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    int c[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = warp; i < ctas; i += 32)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    if ((tid & 31) == 0) s_loss[tid >> 5] = part;
+        for (int k = 0; k < 4; ++k) {
+            const int e = e0 + 32 * k + lane;
+            const long long at = (long long)i * E + min(e, E - 1);
+            s[k] += part_sums[at];
+            c[k] += part_counts[at];
+        }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        s_sum[warp][32 * k + lane] = s[k];
+        s_cnt[warp][32 * k + lane] = c[k];
+    }
+    int v = 0;
+    for (int i = tid; i < ctas; i += kJoinThreads) v += part_live[i];
+    v = __reduce_add_sync(0xffffffffu, v);
+    if (lane == 0) s_live[warp] = v;
+    __syncthreads();
+    double part = 0.0;
+    if (tid < kJoinCols) {
+        float sum = 0.0f;
+        int cnt = 0;
+#pragma unroll
+        for (int w = 0; w < 32; ++w) {
+            sum += s_sum[w][tid];
+            cnt += s_cnt[w][tid];
+        }
+        if (e0 + tid < E) {
+            prob_sums[e0 + tid] = sum;
+            counts[e0 + tid] = cnt;
+            part = (double)cnt * (double)sum;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+        if (lane == 0) s_loss[warp] = part;
+    }
     __syncthreads();
     if (tid == 0) {
-        double total = 0.0;
-        for (int i = 0; i < 32; ++i) total += s_loss[i];
-        const double n = s_live;
-        *n_tokens = s_live;
-        *loss = s_live ? (float)((double)coef * E / (topk * n * n) * total) : 0.0f;
+        cta_loss = 0.0;
+        for (int i = 0; i < kJoinCols / 32; ++i) cta_loss += s_loss[i];
     }
+    cluster.sync();
+    if (blockIdx.x == 0 && tid == 0) {
+        double total = 0.0;
+        int live = 0;
+        for (int k = 0; k < (int)cluster.num_blocks(); ++k)
+            total += *cluster.map_shared_rank(&cta_loss, k);
+        for (int w = 0; w < 32; ++w) live += s_live[w];
+        const double n = live;
+        *n_tokens = live;
+        *loss = live ? (float)((double)coef * E / (topk * n * n) * total) : 0.0f;
+    }
+    cluster.sync();                     // CTA 0 may still read the others' sums
 }
 
 struct BalanceBwdArgs {
@@ -203,77 +269,113 @@ struct BalanceBwdArgs {
     void* dlogits;
 };
 
-template <typename LT, int VPL>
+template <typename LT, int LPT, int NV, bool VEC>
 __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const BalanceBwdArgs a) {
     pdl_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // Since sum_e p_e = 1, c may be taken relative to any constant; relative
-    // to its mean the difference below loses no digits to the common part.
-    float c[VPL];
-    double mean = 0.0;
-#pragma unroll
-    for (int k = 0; k < VPL; ++k)
-        if (32 * k + lane < a.E) mean += a.counts[32 * k + lane];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
-    mean /= a.E;
-#pragma unroll
-    for (int k = 0; k < VPL; ++k)
-        c[k] = 32 * k + lane < a.E ? (float)(a.counts[32 * k + lane] - mean) : 0.0f;
-    const double n = *a.n_tokens;
-    const float factor =
-        n > 0 ? (float)((double)*a.grad_loss * a.coef * a.E / (a.topk * n * n)) : 0.0f;
+    __shared__ float s_factor;
+    constexpr int kSubs = kBalThreads / LPT;
+    const int sub = threadIdx.x / LPT, col = threadIdx.x % LPT;
+    const LT* logits = static_cast<const LT*>(a.logits);
+    auto row_of = [&](long long t) { return logits + min(t, (long long)a.T - 1) * a.ld; };
+    const long long step = (long long)gridDim.x * kSubs;
+    const long long t0 = (long long)blockIdx.x * kSubs + sub;
+    RowRaw<LT, NV> next = load_row<LT, LPT, NV, VEC>(row_of(t0), a.E);
 
-    for (long long t = (long long)blockIdx.x * kBalWarps + warp; t < a.T;
-         t += (long long)gridDim.x * kBalWarps) {
-        LT* out = static_cast<LT*>(a.dlogits) + t * a.E;
-        if (a.mask && !a.mask[t]) {
-            for (int e = lane; e < a.E; e += 32) out[e] = from_f32<LT>(0.0f);
-            continue;
+    // Since sum_e p_e = 1, c may be taken relative to any constant; relative
+    // to its mean (to an integer) the difference below loses no digits to the
+    // part that all counts share.
+    int ci[NV][4];
+    long long total = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int e = 4 * (LPT * i + col) + k;
+            ci[i][k] = e < a.E ? a.counts[e] : 0;
+            total += ci[i][k];
         }
-        float p[VPL], rest[VPL];
-        row_probs<LT, VPL>(static_cast<const LT*>(a.logits) + t * a.ld, a.E, a.sigmoid, p, rest);
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const int mean = (int)(total / a.E);
+    float c[NV][4];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) c[i][k] = (float)(ci[i][k] - mean);
+    if (threadIdx.x == 0) {
+        const double n = *a.n_tokens;
+        s_factor = n > 0 ? (float)((double)*a.grad_loss * a.coef * a.E / (a.topk * n * n)) : 0.0f;
+    }
+    __syncthreads();
+    const float factor = s_factor;
+
+    const long long rounds = (a.T - (long long)blockIdx.x * kSubs + step - 1) / step;
+    for (long long i0 = 0; i0 < rounds; ++i0) {
+        const long long t = t0 + i0 * step;
+        const RowRaw<LT, NV> row = next;
+        if (i0 + 1 < rounds) next = load_row<LT, LPT, NV, VEC>(row_of(t + step), a.E);
+        const bool live = t < a.T && (!a.mask || a.mask[t]);
+        float p[NV][4], rest[NV][4];
+        row_probs<LT, LPT, NV>(row, a.E, a.sigmoid, p, rest);
         float inner = 0.0f;
 #pragma unroll
-        for (int k = 0; k < VPL; ++k) inner = fmaf(p[k], c[k], inner);
-        inner = warp_sum(inner);
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int k = 0; k < VPL; ++k)
-            if (32 * k + lane < a.E)
-                out[32 * k + lane] = from_f32<LT>(p[k] * rest[k] * (c[k] - inner) * factor);
+            for (int k = 0; k < 4; ++k) inner = fmaf(p[i][k], c[i][k], inner);
+        inner = lanes_sum<LPT>(inner);
+        if (t >= a.T) continue;
+        LT* out = static_cast<LT*>(a.dlogits) + t * a.E;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float d[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                d[k] = live ? p[i][k] * rest[i][k] * (c[i][k] - inner) * factor : 0.0f;
+            store4<LT, VEC>(out, 4 * (LPT * i + col), a.E, d);
+        }
     }
 }
 
-int balance_ctas(int T, int sms) {
-    const int want = (int)(((long long)T + kBalWarps * kBalTokensPerWarp - 1) /
-                           (kBalWarps * kBalTokensPerWarp));
-    return std::max(1, std::min(want, sms * 2));
+// Lanes per token and vectors per lane: the fewest lanes that hold a row in one
+// vector each, and from 128 columns on the whole warp.
+#define FERRET_BALANCE_SHAPE(KERNEL, LT, VEC, E, ...)                                   \
+    ((E) <= 32    ? launch_kernel(KERNEL<LT, 8, 1, VEC>, __VA_ARGS__)                   \
+     : (E) <= 64  ? launch_kernel(KERNEL<LT, 16, 1, VEC>, __VA_ARGS__)                  \
+     : (E) <= 128 ? launch_kernel(KERNEL<LT, 32, 1, VEC>, __VA_ARGS__)                  \
+     : (E) <= 256 ? launch_kernel(KERNEL<LT, 32, 2, VEC>, __VA_ARGS__)                  \
+     : (E) <= 512 ? launch_kernel(KERNEL<LT, 32, 4, VEC>, __VA_ARGS__)                  \
+                  : launch_kernel(KERNEL<LT, 32, 8, VEC>, __VA_ARGS__))
+
+// Tokens that a CTA works on at once.
+int balance_tokens(int E) { return kBalThreads / (E <= 32 ? 8 : E <= 64 ? 16 : 32); }
+
+// Two rounds of tokens per CTA before a further CTA pays, four CTAs per SM at most.
+int balance_ctas(int T, int E, int sms) {
+    const int per = 2 * balance_tokens(E);
+    return std::max(1, std::min((int)(((long long)T + per - 1) / per), sms * 4));
 }
 
-// The workspace is sized for the largest device this library runs on, so that
-// the size needs no device: sums and counts [ctas, E], live tokens [ctas].
-constexpr int kBalMaxCtas = 2 * 256;
+// Vector accesses: rows of whole vectors, each on a vector's boundary.
+bool balance_vec(const void* logits, long long ld, int E, int size, const void* out) {
+    return E % 4 == 0 && ld % 4 == 0 && aligned_to(logits, 4 * size) && aligned_to(out, 4 * size);
+}
 
 template <typename LT>
 int run_balance(const BalanceArgs& a, int ctas, cudaStream_t s) {
     const dim3 grid(ctas), block(kBalThreads);
-    const int vpl = (a.E + 31) / 32;
-    if (vpl <= 2) return launch_kernel(moe_balance_kernel<LT, 2>, grid, block, 0, s, a);
-    if (vpl <= 4) return launch_kernel(moe_balance_kernel<LT, 4>, grid, block, 0, s, a);
-    if (vpl <= 8) return launch_kernel(moe_balance_kernel<LT, 8>, grid, block, 0, s, a);
-    if (vpl <= 16) return launch_kernel(moe_balance_kernel<LT, 16>, grid, block, 0, s, a);
-    return launch_kernel(moe_balance_kernel<LT, 32>, grid, block, 0, s, a);
+    return balance_vec(a.logits, a.ld, a.E, sizeof(LT), nullptr)
+               ? FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, true, a.E, grid, block, 0, s, a)
+               : FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, false, a.E, grid, block, 0, s, a);
 }
 
 template <typename LT>
-int run_balance_bwd(const BalanceBwdArgs& a, int ctas, cudaStream_t s) {
-    const dim3 grid(ctas), block(kBalThreads);
-    const int vpl = (a.E + 31) / 32;
-    if (vpl <= 2) return launch_kernel(moe_balance_bwd_kernel<LT, 2>, grid, block, 0, s, a);
-    if (vpl <= 4) return launch_kernel(moe_balance_bwd_kernel<LT, 4>, grid, block, 0, s, a);
-    if (vpl <= 8) return launch_kernel(moe_balance_bwd_kernel<LT, 8>, grid, block, 0, s, a);
-    if (vpl <= 16) return launch_kernel(moe_balance_bwd_kernel<LT, 16>, grid, block, 0, s, a);
-    return launch_kernel(moe_balance_bwd_kernel<LT, 32>, grid, block, 0, s, a);
+int run_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t s) {
+    const int per = balance_tokens(a.E);
+    const dim3 grid((unsigned)std::min<long long>(((long long)a.T + per - 1) / per, sms * 6LL)),
+        block(kBalThreads);
+    return balance_vec(a.logits, a.ld, a.E, sizeof(LT), a.dlogits)
+               ? FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, true, a.E, grid, block, 0, s, a)
+               : FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, false, a.E, grid, block, 0, s, a);
 }
 
 }  // namespace
@@ -283,7 +385,7 @@ using namespace ferret;
 
 extern "C" size_t ferret_moe_balance_loss_workspace_size(int T, int E) {
     if (T <= 0 || E <= 0 || E > kBalMaxE) return 0;
-    return (size_t)balance_ctas(T, kBalMaxCtas / 2) * (2 * (size_t)E + 1) * 4;
+    return (size_t)balance_ctas(T, E, kBalMaxCtas / 4) * (2 * (size_t)E + 1) * 4;
 }
 
 extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dtype,
@@ -307,7 +409,7 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
     int rc = current_device(&info);
     if (rc != FERRET_OK) return rc;
     const cudaStream_t s = as_stream(stream);
-    const int ctas = T ? balance_ctas(T, std::min(info->num_sms, kBalMaxCtas / 2)) : 0;
+    const int ctas = T ? balance_ctas(T, E, std::min(info->num_sms, kBalMaxCtas / 4)) : 0;
     float* sums = static_cast<float*>(workspace);
     int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * E);
     int32_t* live = cnts + (size_t)ctas * E;
@@ -319,8 +421,10 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
                                     : run_balance<float>(a, ctas, s);
         if (rc != FERRET_OK) return rc;
     }
-    return launch_kernel(moe_balance_join_kernel, dim3(1), dim3(1024), 0, s, sums, cnts, live, ctas,
-                         E, topk, coef, loss, counts, prob_sums, n_tokens);
+    const int join = (E + kJoinCols - 1) / kJoinCols;        // at most 8: one cluster
+    return launch_kernel_cluster(moe_balance_join_kernel, dim3(join), dim3(kJoinThreads), 0, join,
+                                 s, sums, cnts, live, ctas, E, topk, coef, loss, counts, prob_sums,
+                                 n_tokens);
 }
 
 extern "C" int ferret_moe_balance_loss_backward(const float* grad_loss, const void* logits,
@@ -340,12 +444,10 @@ extern "C" int ferret_moe_balance_loss_backward(const float* grad_loss, const vo
     if (rc != FERRET_OK) return rc;
     const BalanceBwdArgs a{grad_loss, logits, ld, counts, n_tokens, token_mask, T, E, topk, coef,
                            (flags & FERRET_ROUTE_SIGMOID) != 0, grad_logits};
-    const int ctas = (int)std::min<long long>(((long long)T + kBalWarps - 1) / kBalWarps,
-                                              (long long)info->num_sms * 8);
     const cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case FERRET_BF16: return run_balance_bwd<__nv_bfloat16>(a, ctas, s);
-        case FERRET_FP16: return run_balance_bwd<__half>(a, ctas, s);
-        default: return run_balance_bwd<float>(a, ctas, s);
+        case FERRET_BF16: return run_balance_bwd<__nv_bfloat16>(a, info->num_sms, s);
+        case FERRET_FP16: return run_balance_bwd<__half>(a, info->num_sms, s);
+        default: return run_balance_bwd<float>(a, info->num_sms, s);
     }
 }

@@ -47,12 +47,6 @@ struct RouteArgs {
     int32_t* ids;
 };
 
-// Logits as the selection sees them: closed experts are -inf, +inf is the
-// largest finite value (so that differences stay defined).
-__device__ __forceinline__ float clean_logit(float z) {
-    return z > -INFINITY ? fminf(z, 3.402823466e38f) : -INFINITY;
-}
-
 // sigmoid(z) without cancellation or overflow on either side.
 __device__ __forceinline__ float sigmoid_f(float z) {
     const float e = expf(-fabsf(z));

@@ -12,9 +12,15 @@
 //
 // HBM-bound: a row's x and residual are read once, kept in registers across
 // the reduction, and every output is written once (9 bytes per element with
-// bf16 and all outputs).  One CTA (or one warp, for short rows) owns a row; a
-// thread owns NV chunks of 8 consecutive columns, so a half-warp holds exactly
-// one 128-column block and its amax takes four shuffles.
+// bf16 and all outputs).  A thread owns NV chunks of 8 consecutive columns, so a
+// half-warp holds exactly one 128-column block and its amax takes four shuffles.
+//
+// Two forms.  Few rows, short rows and rows off the 16-byte grid: one CTA (or
+// one warp, for short rows) per row, loads straight to registers.  Many long
+// rows: a persistent grid whose CTAs copy their next rows into a shared-memory
+// ring with bulk copies while they work on the current one; between a row's
+// loads and its stores lies a reduction, and without the ring the memory idles
+// there.
 #include <algorithm>
 
 #include "fp8_quant.cuh"
@@ -98,6 +104,42 @@ __device__ __forceinline__ void load_weight8(const NormArgs& a, int c, int n, fl
     }
 }
 
+// The outputs of a row from its s (v) and the sum of its squares (ss).  All lanes
+// of the warp take part; those without a live row or column store nothing.
+template <typename T, int NV, bool VEC>
+__device__ __forceinline__ void finish_row(const NormArgs& a, long long row, int tid, bool live,
+                                           const float (&v)[NV][8], float ss) {
+    const int tpr = a.tpr, K = a.K;
+    const float inv = 1.0f / sqrtf(ss / (float)K + a.eps);
+
+    const int nk = K >> 7;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = i * tpr + tid, n = live ? K - c * 8 : 0;
+        float y[8];
+        float amax = 0.0f;
+        if (n > 0) {
+            if (a.residual_out)
+                store8<T, VEC>(static_cast<T*>(a.residual_out) + row * K + c * 8, n, v[i]);
+            float w[8];
+            load_weight8<T, VEC>(a, c, n, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inv * w[j];
+            if (a.y) store8<T, VEC>(static_cast<T*>(a.y) + row * K + c * 8, n, y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
+        }
+        if (!a.q) continue;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)          // within the 16 lanes of a 128-column block
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (n <= 0) continue;
+        const Fp8Scale f = fp8_block_scale(amax, a.ue8m0);
+        *reinterpret_cast<uint2*>(a.q + row * K + c * 8) = fp8_pack8(y, f.mul);
+        if ((tid & 15) == 0) a.scale[row * nk + (c >> 4)] = f.scale;
+    }
+}
+
 // VEC: K is a multiple of 8 and every row of x, residual, weight, y and
 // residual_out starts on a 16-byte boundary; otherwise elements move one by one.
 template <typename T, int NV, bool VEC>
@@ -140,34 +182,91 @@ __global__ void __launch_bounds__(kNormMaxThreads) add_rms_norm_kernel(const Nor
         ss = (threadIdx.x & 31) < (tpr >> 5) ? warp_sums[threadIdx.x & 31] : 0.0f;
         ss = warp_sum(ss);
     }
-    const float inv = 1.0f / sqrtf(ss / (float)K + a.eps);
+    finish_row<T, NV, VEC>(a, row, tid, live, v, ss);
+}
 
-    const int nk = K >> 7;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = i * tpr + tid, n = live ? K - c * 8 : 0;
-        float y[8];
-        float amax = 0.0f;
-        if (n > 0) {
-            if (a.residual_out)
-                store8<T, VEC>(static_cast<T*>(a.residual_out) + row * K + c * 8, n, v[i]);
-            float w[8];
-            load_weight8<T, VEC>(a, c, n, w);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inv * w[j];
-            if (a.y) store8<T, VEC>(static_cast<T*>(a.y) + row * K + c * 8, n, y);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
-        }
-        if (!a.q) continue;
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1)          // within the 16 lanes of a 128-column block
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (n <= 0) continue;
-        const Fp8Scale f = fp8_block_scale(amax, a.ue8m0);
-        *reinterpret_cast<uint2*>(a.q + row * K + c * 8) = fp8_pack8(y, f.mul);
-        if ((tid & 15) == 0) a.scale[row * nk + (c >> 4)] = f.scale;
+// --------------------------------------------------------- the persistent form
+
+constexpr int kRingMax = 4;
+
+// Stage layout: x row, then the residual row (K elements each, 16-byte multiple).
+template <typename T, int NV>
+__global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const NormArgs a, int stages,
+                                                                const DevCtl ctl) {
+    pdl_begin();
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ float warp_sums[2][16];
+    __shared__ uint64_t full[kRingMax];
+    __shared__ int abort_flag;
+    const int tid = threadIdx.x, tpr = a.tpr, K = a.K, lane = tid & 31;
+    const uint32_t row_bytes = (uint32_t)K * sizeof(T);
+    const uint32_t stage_bytes = a.residual ? 2 * row_bytes : row_bytes;
+    if (tid == 0) {
+        for (int i = 0; i < stages; ++i) mbar_init(smem_addr(&full[i]), 1);
+        abort_flag = 0;
+        mbar_init_fence();
     }
+    __syncthreads();
+    auto fetch = [&](int slot, long long row) {            // thread 0
+        const uint32_t bar = smem_addr(&full[slot]), dst = smem_addr(ring) + slot * stage_bytes;
+        mbar_expect_tx(bar, stage_bytes);
+        const uint64_t policy = policy_evict_first();
+        bulk_load_hint(dst, static_cast<const T*>(a.x) + row * a.ldx, row_bytes, bar, policy);
+        if (a.residual)
+            bulk_load_hint(dst + row_bytes, static_cast<const T*>(a.residual) + row * a.ldr,
+                           row_bytes, bar, policy);
+    };
+    const long long step = gridDim.x;
+    if (tid == 0)
+        for (int i = 0; i < stages && blockIdx.x + i * step < a.T; ++i)
+            fetch(i, blockIdx.x + i * step);
+
+    RingPos pos;
+    int odd = 0;
+    for (long long row = blockIdx.x; row < a.T; row += step, odd ^= 1) {
+        const bool ok = mbar_wait(smem_addr(&full[pos.slot]), pos.phase, &abort_flag, ctl, 22);
+        const uint8_t* stage = ring + pos.slot * stage_bytes;
+        float v[NV][8];
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = i * tpr + tid;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+            if (c * 8 >= K) continue;
+            Raw8<T> raw;
+            const uint4* p = reinterpret_cast<const uint4*>(stage + (size_t)c * 8 * sizeof(T));
+#pragma unroll
+            for (int j = 0; j < (int)(sizeof(T) / 2); ++j) raw.w[j] = p[j];
+            unpack8<T>(raw, v[i]);
+            if (a.residual) {
+                float r[8];
+                p = reinterpret_cast<const uint4*>(stage + row_bytes + (size_t)c * 8 * sizeof(T));
+#pragma unroll
+                for (int j = 0; j < (int)(sizeof(T) / 2); ++j) raw.w[j] = p[j];
+                unpack8<T>(raw, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+        }
+        ss = warp_sum(ss);
+        if (lane == 0) warp_sums[odd][tid >> 5] = ss;
+        // every thread has the row in registers: the stage is free again
+        if (__syncthreads_or(!ok)) break;
+        if (tid == 0 && row + stages * step < a.T) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            fetch(pos.slot, row + stages * step);
+        }
+        pos.advance(stages);
+        ss = warp_sum(lane < (tpr >> 5) ? warp_sums[odd][lane] : 0.0f);
+        finish_row<T, NV, true>(a, row, tid, true, v, ss);
+    }
+    // a wait ran out: let the copies in flight land before the CTA leaves
+    if (abort_flag && tid == 0)
+        for (int i = 0; i < stages; ++i, pos.advance(stages))
+            mbar_wait(smem_addr(&full[pos.slot]), pos.phase, &abort_flag, ctl, 22, false);
 }
 
 template <typename T, int NV>
@@ -178,9 +277,23 @@ int launch_norm(const NormArgs& a, bool vec, int threads, cudaStream_t s) {
                : launch_kernel(add_rms_norm_kernel<T, NV, false>, grid, dim3(threads), 0, s, a);
 }
 
+template <typename T, int NV>
+int launch_ring(const NormArgs& a, int ctas_per_sm, int stages, size_t smem, const DeviceInfo* info,
+                cudaStream_t s) {
+    auto kern = add_rms_norm_ring_kernel<T, NV>;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
+            cudaSuccess) {
+        cudaGetLastError();
+        return FERRET_ERR_CUDA;
+    }
+    const dim3 grid((unsigned)std::min<long long>(a.T, (long long)info->num_sms * ctas_per_sm));
+    return launch_kernel(kern, grid, dim3(a.tpr), smem, s, a, stages, make_ctl(info));
+}
+
 template <typename T>
-int run_norm(NormArgs& a, bool vec, int sms, cudaStream_t s) {
-    const int chunks = (a.K + 7) / 8;
+int run_norm(NormArgs& a, bool vec, const DeviceInfo* info, cudaStream_t s) {
+    const int chunks = (a.K + 7) / 8, sms = info->num_sms;
     if (chunks <= 32 * kNormMaxNV && a.T > sms * 8) {
         // short rows, many of them: a warp (or half of one) per row, 8 warps per CTA
         const int nv = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
@@ -188,6 +301,18 @@ int run_norm(NormArgs& a, bool vec, int sms, cudaStream_t s) {
         return nv == 1   ? launch_norm<T, 1>(a, vec, 256, s)
                : nv == 2 ? launch_norm<T, 2>(a, vec, 256, s)
                          : launch_norm<T, 4>(a, vec, 256, s);
+    }
+    // Many long rows: the ring, with at least three rows in it.  An SM has 1 KB of
+    // shared memory more than a CTA may use; a CTA takes 1 KB besides its own.
+    const size_t stage = (size_t)a.K * sizeof(T) * (a.residual ? 2 : 1);
+    const int room = info->max_smem_optin + 1024, own = 1024 + 512;
+    if (vec && a.T > sms * 8 && chunks <= 2 * 512 && 3 * stage + own <= (size_t)room) {
+        const int nv = chunks <= 256 ? 1 : 2;
+        a.tpr = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+        const int ctas = std::min(2048 / a.tpr / 2, (int)(room / (3 * stage + own)));
+        const int stages = std::min<int>(kRingMax, (int)((room / ctas - own) / stage));
+        return nv == 1 ? launch_ring<T, 1>(a, ctas, stages, stage * stages, info, s)
+                       : launch_ring<T, 2>(a, ctas, stages, stage * stages, info, s);
     }
     // few rows: one chunk per thread (shortest path through a row); many: more
     // chunks per thread, so that more rows are in flight on an SM
@@ -232,8 +357,8 @@ extern "C" int ferret_add_rms_norm(const void* x, long long ldx, const void* res
                (flags & FERRET_UE8M0_SCALES) != 0, 0};
     const cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case FERRET_BF16: return run_norm<__nv_bfloat16>(a, vec, info->num_sms, s);
-        case FERRET_FP16: return run_norm<__half>(a, vec, info->num_sms, s);
-        default: return run_norm<float>(a, vec, info->num_sms, s);
+        case FERRET_BF16: return run_norm<__nv_bfloat16>(a, vec, info, s);
+        case FERRET_FP16: return run_norm<__half>(a, vec, info, s);
+        default: return run_norm<float>(a, vec, info, s);
     }
 }

@@ -64,17 +64,71 @@ __device__ __forceinline__ Raw8<T> pack8(const float v[8]) {
     return r;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Four consecutive elements of a row, VEC: as one aligned load; else element by
+// element with indices clamped into the row of n (the caller discards what lies
+// behind it).
+template <typename T, bool VEC>
+__device__ __forceinline__ void load4(const T* row, int at, int n, T v[4]) {
+    if (VEC) {
+        if (sizeof(T) == 4) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(row + min(at, n - 4)));
+            memcpy(v, &w, 16);
+        } else {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(row + min(at, n - 4)));
+            memcpy(v, &w, 8);
+        }
+    } else {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int i = 0; i < 4; ++i) v[i] = row[min(at + i, n - 1)];
+    }
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store4(T* row, int at, int n, const float v[4]) {
+    T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(v[i]);
+    if (VEC) {
+        if (at >= n) return;
+        if (sizeof(T) == 4) {
+            uint4 w;
+            memcpy(&w, e, 16);
+            *reinterpret_cast<uint4*>(row + at) = w;
+        } else {
+            uint2 w;
+            memcpy(&w, e, 8);
+            *reinterpret_cast<uint2*>(row + at) = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < n) row[at + i] = e[i];
+    }
+}
+
+// Logits as the row kernels see them: NaN closes an expert like -inf, +inf is
+// the largest finite value (so that differences stay defined).
+__device__ __forceinline__ float clean_logit(float z) {
+    return z > -INFINITY ? fminf(z, 3.402823466e38f) : -INFINITY;
+}
+
+// Reductions over the lanes of aligned groups of N lanes.
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = N / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+
+__device__ __forceinline__ float warp_sum(float v) { return lanes_sum<32>(v); }
+__device__ __forceinline__ float warp_max(float v) { return lanes_max<32>(v); }
 
 }  // namespace
 

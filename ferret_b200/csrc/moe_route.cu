@@ -14,18 +14,25 @@
 // weight 0, which the permutation and the combine skip.
 //
 // Which of two keys is larger decides an integer, so the order has to be that
-// of the exact keys.  Without a bias the score is monotone in z and z itself
-// is compared.  Otherwise keys carry the rounding of exp and of the sum; the
-// selection runs on fp32 keys and also looks at the gap between each chosen
-// key and the next: a gap below the bound on that rounding sends the token to
-// a second selection with keys in fp64 (under one token in a hundred).
+// of the exact keys.  The selection runs on approximate keys (fast fp32
+// scores, the low bits of a key's integer image traded for the expert's place in
+// its lane) and looks at the gap between each chosen key and the next: where
+// a gap is below the bound on the approximation and the two experts are not
+// equal by their inputs, the token takes a second selection with keys in fp64
+// (under one token in a hundred).  Without a bias the score is monotone in z,
+// and z itself is the key.
 //
-// HBM-bound at large T (the logits are read once), latency-bound at small T.
-// One warp per token with the keys in registers: a round of the choice is a
-// compare of a lane's keys plus two warp reductions (redux.sync) on an
-// order-preserving integer image of the key.  Groups are whole lane segments
-// (n_group is a power of two), so a group's best two keys need
-// log2(32 / n_group) shuffles.
+// HBM-bound at large T (the logits are read once), latency-bound at small T; in
+// between the instructions of the selection bound it.  One warp per token, the
+// keys of a lane in registers, sorted once (a merge-sorting network of the
+// lane's keys).  A round of the choice is then one warp maximum (redux.sync) of
+// the lanes' heads, a ballot that finds the lowest lane that has it, and a shift of
+// that lane's list; the gaps are looked at once, after the rounds, by all
+// slots together.  Lanes hold consecutive experts and groups are whole lane
+// segments (n_group is a power of two), so the lowest lane has the lowest id, and
+// a group's best two keys need log2(32 / n_group) shuffles.
+#include <algorithm>
+
 #include "row_io.cuh"
 
 namespace ferret {
@@ -41,7 +48,10 @@ struct RouteArgs {
     const float* bias;
     const uint8_t* mask;
     int T, E, topk, n_group, topk_group, group_top;
+    int lpg_log;          // log2 of the lanes per group
+    int slots_log;        // log2 of the lanes per token of the last step (2^slots_log >= topk)
     bool sigmoid, renorm;
+    bool bare;            // z orders the experts
     float scale;
     float* weights;
     int32_t* ids;
@@ -57,22 +67,40 @@ __device__ __forceinline__ double sigmoid_d(double z) {
     return (z >= 0.0 ? 1.0 : e) / (1.0 + e);
 }
 
-// Order-preserving image of a float: a < b <=> order(a) < order(b), -0 == +0.
-__device__ __forceinline__ unsigned order_of(float v) {
-    const unsigned u = __float_as_uint(v + 0.0f);
-    return u ^ ((int)u < 0 ? 0xffffffffu : 0x80000000u);
-}
-__device__ __forceinline__ float value_of(unsigned o) {
-    return __uint_as_float(o ^ ((int)o < 0 ? 0x80000000u : 0xffffffffu));
+// Fast sigmoid for keys, within 2^-21: ex2 (relative error 2^-22; the rounding of
+// its argument weighs |z| e^-|z| 2^-23) and reciprocal (1 ulp) approximations.
+__device__ __forceinline__ float sigmoid_key(float z) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return r;
 }
 
-// The largest v over the warp, and the smallest idx among the lanes that have it.
-__device__ __forceinline__ void warp_best(float& v, int& idx) {
-    const unsigned o = order_of(v);
-    const unsigned m = __reduce_max_sync(kFull, o);
-    idx = (int)__reduce_min_sync(kFull, o == m ? (unsigned)idx : 0x7fffffffu);
-    v = value_of(m);
+// Order-preserving image of a float that is not -0: a < b <=> order(a) < order(b).
+// No float above -inf maps to 0, which stands for a closed expert.
+__device__ __forceinline__ unsigned order_of(float v) {
+    const int u = __float_as_int(v);
+    return (unsigned)(u ^ ((u >> 31) | (int)0x80000000));
 }
+__device__ __forceinline__ float value_of(unsigned o) {
+    const int u = (int)~o;
+    return __int_as_float((int)o ^ ((u >> 31) | (int)0x80000000));
+}
+
+// Where a lane's experts are: `n` of its group's (lane >> lpg_log) from `base` on.
+struct Span {
+    int base, n;
+};
+
+__device__ __forceinline__ Span lane_span(const RouteArgs& a) {
+    const int lane = threadIdx.x & 31, lpg = 1 << a.lpg_log, G = a.E / a.n_group;
+    const int vpl = (G + lpg - 1) >> a.lpg_log, off = (lane & (lpg - 1)) * vpl;
+    return {(lane >> a.lpg_log) * G + off, max(0, min(vpl, G - off))};
+}
+
+// ---- the selection with keys in fp64, for tokens whose approximate keys are too
+// close: plain rounds over the lane's keys
+
 __device__ __forceinline__ void warp_best(double& v, int& idx) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -82,97 +110,10 @@ __device__ __forceinline__ void warp_best(double& v, int& idx) {
     }
 }
 
-// Where a lane's experts are: group lane / lpg, `n` of them from `base` on.
-struct Span {
-    int base, n;
-};
-
-__device__ __forceinline__ Span lane_span(int E, int n_group) {
-    const int lane = threadIdx.x & 31, lpg = 32 / n_group, G = E / n_group;
-    const int vpl = (G + lpg - 1) / lpg, off = (lane % lpg) * vpl;
-    return {lane / lpg * G + off, max(0, min(vpl, G - off))};
-}
-
-// Closes the keys of all but the topk_group best groups.  Returns true if the
-// border between the last open and the first closed group is closer than tol.
-template <typename F, int VPL>
-__device__ __forceinline__ bool close_groups(F (&key)[VPL], const RouteArgs& a, F tol) {
-    const int lane = threadIdx.x & 31, lpg = 32 / a.n_group;
-    F b1 = -INFINITY, b2 = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        b2 = fmax(b2, fmin(b1, key[k]));
-        b1 = fmax(b1, key[k]);
-    }
-    for (int o = 1; o < lpg; o <<= 1) {
-        const F c1 = __shfl_xor_sync(kFull, b1, o), c2 = __shfl_xor_sync(kFull, b2, o);
-        b2 = fmax(fmin(b1, c1), fmax(b2, c2));
-        b1 = fmax(b1, c1);
-    }
-    F score = b1;
-    if (a.group_top == 2 && b2 > -INFINITY) score += b2;
-    bool open = false;
-    F last = INFINITY;
-    bool near = false;
-    for (int i = 0; i <= a.topk_group && i < a.n_group; ++i) {
-        F v = open ? (F)-INFINITY : score;
-        int g = lane / lpg;
-        warp_best(v, g);
-        if (!(v > -INFINITY)) break;
-        if (i == a.topk_group) {
-            near = last - v <= tol;
-            break;
-        }
-        if (g == lane / lpg) open = true;
-        last = v;
-    }
-    if (!open)
-#pragma unroll
-        for (int k = 0; k < VPL; ++k) key[k] = -INFINITY;
-    return near;
-}
-
-template <typename LT>
-__device__ __forceinline__ bool same_expert(const RouteArgs& a, const LT* row, int i, int j) {
-    return clean_logit(to_f32(row[i])) == clean_logit(to_f32(row[j])) &&
-           (!a.bias || a.bias[i] == a.bias[j]);
-}
-
-// Picks up to topk experts; lane j gets the id of slot j (-1: none left).
-// With tol >= 0 the gaps down to the first key not chosen are watched: returns
-// true where one is within tol and the two experts are not equal by input.
-template <typename F, int VPL, typename LT>
-__device__ __forceinline__ bool pick(F (&key)[VPL], const Span sp, const RouteArgs& a,
-                                     const LT* row, F tol, int& my_id) {
-    const int lane = threadIdx.x & 31;
-    F last = INFINITY;
-    int last_id = -1;
-    my_id = -1;
-    const int rounds = a.topk + (tol >= 0 ? 1 : 0);
-    for (int j = 0; j < rounds; ++j) {
-        F v = -INFINITY;
-        int k0 = 0;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k)
-            if (key[k] > v) v = key[k], k0 = k;
-        int id = sp.base + k0;
-        warp_best(v, id);
-        if (!(v > -INFINITY)) break;
-        if (tol >= 0 && j > 0 && last - v <= tol && !same_expert(a, row, last_id, id)) return true;
-#pragma unroll
-        for (int k = 0; k < VPL; ++k)
-            if (sp.base + k == id && k < sp.n) key[k] = -INFINITY;
-        if (j == lane && j < a.topk) my_id = id;
-        last = v;
-        last_id = id;
-    }
-    return false;
-}
-
-// The selection with keys in fp64, for tokens whose fp32 keys are too close.
 template <typename LT, int VPL>
 __device__ __noinline__ int pick_exact(const RouteArgs& a, const LT* row) {
-    const Span sp = lane_span(a.E, a.n_group);
+    const Span sp = lane_span(a);
+    const int lane = threadIdx.x & 31, lpg = 1 << a.lpg_log, group = lane >> a.lpg_log;
     double key[VPL];
     double m = -INFINITY, sum = 0.0;
 #pragma unroll
@@ -180,98 +121,361 @@ __device__ __noinline__ int pick_exact(const RouteArgs& a, const LT* row) {
         key[k] = k < sp.n ? (double)clean_logit(to_f32(row[sp.base + k])) : -INFINITY;
         m = fmax(m, key[k]);
     }
-    if (!a.sigmoid) {
-        int unused = 0;
-        warp_best(m, unused);
+    if (!a.bare) {
+        if (!a.sigmoid) {
+            int unused = 0;
+            warp_best(m, unused);
 #pragma unroll
-        for (int k = 0; k < VPL; ++k) sum += key[k] > -INFINITY ? exp(key[k] - m) : 0.0;
+            for (int k = 0; k < VPL; ++k) sum += key[k] > -INFINITY ? exp(key[k] - m) : 0.0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
-    }
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+        }
 #pragma unroll
-    for (int k = 0; k < VPL; ++k) {
-        if (!(key[k] > -INFINITY)) continue;
-        key[k] = a.sigmoid ? sigmoid_d(key[k]) : exp(key[k] - m) / sum;
-        if (a.bias) {
-            key[k] += (double)a.bias[sp.base + k];
-            if (!(key[k] > -INFINITY)) key[k] = -INFINITY;
+        for (int k = 0; k < VPL; ++k) {
+            if (!(key[k] > -INFINITY)) continue;
+            key[k] = a.sigmoid ? sigmoid_d(key[k]) : exp(key[k] - m) / sum;
+            if (a.bias) {
+                key[k] += (double)a.bias[sp.base + k];
+                if (!(key[k] > -INFINITY)) key[k] = -INFINITY;
+            }
         }
     }
-    if (a.n_group > 1) close_groups<double, VPL>(key, a, -1.0);
-    int id;
-    pick<double, VPL>(key, sp, a, row, -1.0, id);
-    return id;
+    if (a.n_group > 1) {
+        double b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) {
+            b2 = fmax(b2, fmin(b1, key[k]));
+            b1 = fmax(b1, key[k]);
+        }
+        for (int o = 1; o < lpg; o <<= 1) {
+            const double c1 = __shfl_xor_sync(kFull, b1, o), c2 = __shfl_xor_sync(kFull, b2, o);
+            b2 = fmax(fmin(b1, c1), fmax(b2, c2));
+            b1 = fmax(b1, c1);
+        }
+        double score = b1;
+        if (a.group_top == 2 && b2 > -INFINITY) score += b2;
+        bool open = false;
+        for (int i = 0; i < a.topk_group; ++i) {
+            double v = open ? -INFINITY : score;
+            int g = group;
+            warp_best(v, g);
+            if (v > -INFINITY && g == group) open = true;
+        }
+        if (!open)
+#pragma unroll
+            for (int k = 0; k < VPL; ++k) key[k] = -INFINITY;
+    }
+    int my_id = -1;
+    for (int j = 0; j < a.topk; ++j) {
+        double v = -INFINITY;
+        int id = sp.base;
+#pragma unroll
+        for (int k = 0; k < VPL; ++k)
+            if (key[k] > v) v = key[k], id = sp.base + k;
+        warp_best(v, id);
+        if (!(v > -INFINITY)) break;
+#pragma unroll
+        for (int k = 0; k < VPL; ++k)
+            if (sp.base + k == id && k < sp.n) key[k] = -INFINITY;
+        if (j == lane) my_id = id;
+    }
+    return my_id;
 }
 
-template <typename LT, int VPL>
-__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(const RouteArgs a) {
-    pdl_begin();
+// Orders n <= 32 candidates (ids) by their exact keys and returns slot lane's: for
+// tokens whose groups are settled.  One candidate per lane; its place is the number
+// of candidates before it.
+template <typename LT>
+__device__ __noinline__ int order_exact(const RouteArgs& a, const LT* row, int* ids, int n) {
     const int lane = threadIdx.x & 31;
-    const Span sp = lane_span(a.E, a.n_group);
-    const bool bare = !a.bias && (a.n_group == 1 || a.group_top == 1);   // z orders the experts
-    for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T;
-         t += (long long)gridDim.x * kRouteWarps) {
-        const LT* row = static_cast<const LT*>(a.logits) + t * a.ld;
+    const int id = lane < n ? ids[lane] : -1;
+    double key = id >= 0 ? (double)clean_logit(to_f32(row[id])) : -INFINITY;
+    if (!a.bare) {
+        if (a.sigmoid) {
+            if (id >= 0) key = sigmoid_d(key);
+        } else {
+            float m = -INFINITY;
+            for (int e = lane; e < a.E; e += 32) m = fmaxf(m, clean_logit(to_f32(row[e])));
+            m = warp_max(m);
+            double sum = 0.0;
+            for (int e = lane; e < a.E; e += 32)
+                sum += exp((double)clean_logit(to_f32(row[e])) - (double)m);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kFull, sum, o);
+            if (id >= 0) key = exp(key - (double)m) / sum;
+        }
+        if (a.bias && id >= 0) key += (double)a.bias[id];
+    }
+    int place = 0;
+    for (int i = 0; i < n; ++i) {
+        const double other = __shfl_sync(kFull, key, i);
+        const int other_id = __shfl_sync(kFull, id, i);
+        place += other > key || (other == key && other_id < id);
+    }
+    __syncwarp();
+    if (id >= 0) ids[place] = id;
+    __syncwarp();
+    return lane < min(n, a.topk) ? ids[lane] : -1;
+}
+
+// ---- the usual selection
+
+__device__ __forceinline__ void sort_two(unsigned& a, unsigned& b) {
+    const unsigned hi = max(a, b);
+    b = min(a, b);
+    a = hi;
+}
+
+// Descending odd-even merge sort (Batcher) of N registers, N a power of two.
+template <int N>
+__device__ __forceinline__ void sort_down(unsigned (&v)[N]) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int q = p; q > 0; q /= 2)
+#pragma unroll
+            for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+                for (int i = 0; i < q; ++i)
+                    if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p))
+                        sort_two(v[i + j], v[i + j + q]);
+}
+
+// A lane's logits as loaded.
+template <typename LT, int VPL>
+struct LaneRow {
+    LT e[VPL];
+};
+
+// VEC: the lane holds exactly VPL experts, at a vector's boundary.
+template <typename LT, int VPL, bool VEC>
+__device__ __forceinline__ LaneRow<LT, VPL> load_lane(const LT* row, const Span sp, int E) {
+    LaneRow<LT, VPL> r;
+    if (VEC) {
+#pragma unroll
+        for (int k = 0; k < VPL / 4; ++k) {
+            LT v[4];
+            load4<LT, true>(row, sp.base + 4 * k, E, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.e[4 * k + i] = v[i];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < VPL; ++k) r.e[k] = row[min(sp.base + k, E - 1)];
+    }
+    return r;
+}
+
+template <typename LT, int VPL, bool VEC>
+__global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
+    moe_route_kernel(const __grid_constant__ RouteArgs a) {
+    pdl_begin();
+    __shared__ int picked[kRouteWarps][33];      // the ids in the order of the rounds
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned below = (1u << lane) - 1u;
+    const Span sp = lane_span(a);
+    const LT* logits = static_cast<const LT*>(a.logits);
+    // A warp takes runs of `per` tokens; their weights are computed together, lane
+    // (i << slots_log) + j for slot j of token i.
+    const int per = 32 >> a.slots_log;
+    const long long step = ((long long)gridDim.x * kRouteWarps - 1) * per;   // past a run
+    long long t = ((long long)blockIdx.x * kRouteWarps + warp) * per;
+    if (t >= a.T) return;
+    LaneRow<LT, VPL> next = load_lane<LT, VPL, VEC>(logits + t * a.ld, sp, a.E);
+    float bias[VPL];
+    float size = 1.0f;                            // no key is larger (unless z is the key)
+#pragma unroll
+    for (int k = 0; k < VPL; ++k) {
+        bias[k] = a.bias ? a.bias[min(sp.base + k, a.E - 1)] : 0.0f;
+        if (fabsf(bias[k]) < INFINITY) size = fmaxf(size, 1.0f + fabsf(bias[k]));
+    }
+    size = warp_max(size);
+    // Two keys further apart than abs_off + rel * size are in their exact order.
+    // A key may be off by a part of its size (the bits that give way to the
+    // place in the lane, the rounding of the sum with the bias) and by a part
+    // of its score, which is at most 1: the fast sigmoid by less than 2^-21, the softmax (VPL + 5 additions in the
+    // sum, the exponentials, the quotient) by (VPL + 16) 2^-24.
+    const float rel = 2.0f * (VPL + 2) * 0x1p-23f;
+    const float abs_off = a.bare ? 0.0f : 2.0f * (a.sigmoid ? 0x1p-21f : (VPL + 16) * 0x1p-24f);
+    // A key's integer image with its place in the lane, 0 for a closed expert
+    // (bias 0 turns -0 into +0; the largest finite value stands for +inf).
+    auto image = [&](float v, int k, bool open) {
+        v = fminf(v, 3.402823466e38f);
+        const unsigned o = (order_of(v) & ~(unsigned)(VPL - 1)) | (unsigned)(VPL - 1 - k);
+        return open && v > -INFINITY && (VEC || k < sp.n) ? o : 0u;
+    };
+    int in_run = 0, run_id = -1;
+    float run_m = 0.0f, run_sum = 1.0f;
+    while (t < a.T) {
+        const LT* row = logits + t * a.ld;
+        const LaneRow<LT, VPL> raw = next;
+        const long long t_next = t + 1 + (in_run + 1 == per ? step : 0);
+        if (t_next < a.T) next = load_lane<LT, VPL, VEC>(logits + t_next * a.ld, sp, a.E);
         int id = -1;
         float m = -INFINITY, sum = 0.0f;
         if (!a.mask || a.mask[t]) {
-            float key[VPL];
-#pragma unroll
-            for (int k = 0; k < VPL; ++k) {
-                key[k] = k < sp.n ? clean_logit(to_f32(row[sp.base + k])) : -INFINITY;
-                m = fmaxf(m, key[k]);
-            }
-            m = warp_max(m);
-            // Two keys further apart than tol are in their exact order: a
-            // sigmoid is within 2^-22 of the exact one (expf 2 ulp, two
-            // roundings), a softmax within (VPL + 12) 2^-24 (VPL + 5 additions
-            // in the sum, expf, the division), and the sum with the bias adds
-            // half an ulp of the key.
-            float tol = -1.0f;
-            if (m > -INFINITY && !a.sigmoid && (!bare || !a.renorm)) {
-#pragma unroll
-                for (int k = 0; k < VPL; ++k)
-                    sum += key[k] > -INFINITY ? expf(key[k] - m) : 0.0f;
-                sum = warp_sum(sum);
-            }
-            if (!bare) {
-                float big = 1.0f;
+            unsigned list[VPL];
+            if (a.sigmoid && !a.bare) {
 #pragma unroll
                 for (int k = 0; k < VPL; ++k) {
-                    if (!(key[k] > -INFINITY)) continue;
-                    key[k] = a.sigmoid ? sigmoid_f(key[k]) : expf(key[k] - m) / sum;
-                    if (a.bias) {
-                        key[k] += a.bias[sp.base + k];
-                        if (!(key[k] > -INFINITY)) key[k] = -INFINITY;
-                        if (fabsf(key[k]) < INFINITY) big = fmaxf(big, fabsf(key[k]));
+                    const float z = to_f32(raw.e[k]);
+                    list[k] = image(sigmoid_key(z) + bias[k], k, z > -INFINITY);
+                }
+            } else {
+                float z[VPL], e[VPL];
+#pragma unroll
+                for (int k = 0; k < VPL; ++k) {
+                    z[k] = clean_logit(to_f32(raw.e[k]));
+                    if (!VEC && k >= sp.n) z[k] = -INFINITY;
+                    e[k] = z[k];
+                }
+                if (!a.sigmoid && (!a.bare || !a.renorm)) {
+#pragma unroll
+                    for (int k = 0; k < VPL; ++k) m = fmaxf(m, z[k]);
+                    m = warp_max(m);
+                    const float shift = m > -INFINITY ? m : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < VPL; ++k) {
+                        e[k] = expf(z[k] - shift);
+                        sum += e[k];
+                    }
+                    sum = warp_sum(sum);
+                    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < VPL; ++k) e[k] = a.bare ? z[k] : e[k] * inv;
+                }
+#pragma unroll
+                for (int k = 0; k < VPL; ++k)
+                    list[k] = image(e[k] + bias[k], k, z[k] > -INFINITY);
+            }
+            sort_down<VPL>(list);
+            bool near = false;
+            if (a.n_group > 1) {
+                const int lpg = 1 << a.lpg_log;
+                unsigned b1 = list[0], b2 = VPL > 1 ? list[1] : 0u;
+                for (int o = 1; o < lpg; o <<= 1) {
+                    const unsigned c1 = __shfl_xor_sync(kFull, b1, o),
+                                   c2 = __shfl_xor_sync(kFull, b2, o);
+                    b2 = max(min(b1, c1), max(b2, c2));
+                    b1 = max(b1, c1);
+                }
+                float sc = value_of(b1);
+                if (a.group_top == 2 && b2) sc += value_of(b2);
+                // Distinct images: the lower group first among equals.  A group
+                // is open if fewer than topk_group come before it.
+                const int group = lane >> a.lpg_log;
+                const unsigned score = b1 ? (order_of(sc) & ~31u) | (31 - group) : 31u - group;
+                int before = 0;
+#pragma unroll 4
+                for (int g = 0; g < 32; g += lpg) before += __shfl_sync(kFull, score, g) > score;
+                const bool open = before < a.topk_group;
+                if (!open)
+#pragma unroll
+                    for (int k = 0; k < VPL; ++k) list[k] = 0u;
+                // the border between open and closed groups: two sums of two keys,
+                // rounded, with five bits given away
+                const unsigned lo = __reduce_min_sync(kFull, open ? score : 0xffffffffu);
+                const unsigned hi = __reduce_max_sync(kFull, open ? 0u : score);
+                if (hi > 31u) {
+                    const float vl = value_of(lo), vh = value_of(hi);
+                    const float big = a.bare ? fmaxf(fabsf(vl), fabsf(vh)) : size;
+                    near = vl - vh <= 2.0f * abs_off + (2.0f * rel + 70 * 0x1p-23f) * big;
+                }
+            }
+            unsigned mine = 0u, more = 0u;        // slot lane's key; the first key not chosen
+            for (int j = 0; j <= a.topk; ++j) {
+                // equal keys: the lowest lane, and in it the lowest place (sorted first)
+                const unsigned head = list[0] & ~(unsigned)(VPL - 1);
+                const unsigned best = __reduce_max_sync(kFull, head);
+                const unsigned have = __ballot_sync(kFull, head == best);
+                if (head == best && !(have & below)) {
+                    picked[warp][j] = sp.base + VPL - 1 - (int)(list[0] & (VPL - 1));
+#pragma unroll
+                    for (int k = 0; k + 1 < VPL; ++k) list[k] = list[k + 1];
+                    list[VPL - 1] = 0u;
+                }
+                if (j == lane) mine = best;
+                more = best;
+            }
+            __syncwarp();
+            // slot lane against the one after it
+            const unsigned down = __shfl_down_sync(kFull, mine, 1);
+            const unsigned after = lane == a.topk - 1 ? more : down;
+            bool close = false;
+            if (lane < a.topk && mine) {
+                id = picked[warp][lane];
+                if (after) {
+                    const float v = value_of(mine), w = value_of(after);
+                    const float big = a.bare ? fmaxf(fabsf(v), fabsf(w)) : size;
+                    if (v - w <= abs_off + rel * big) {
+                        const int other = picked[warp][lane + 1];
+                        close = clean_logit(to_f32(row[id])) != clean_logit(to_f32(row[other])) ||
+                                (a.bias && a.bias[id] != a.bias[other]);
                     }
                 }
-                tol = (a.sigmoid ? 0x1p-20f : (VPL + 12) * 0x1p-23f) + 0x1p-22f * warp_max(big);
             }
-            bool near = false;
-            if (a.n_group > 1) near = close_groups<float, VPL>(key, a, bare ? -1.0f : 2.0f * tol);
-            if (!near) near = pick<float, VPL>(key, sp, a, row, tol, id);
-            if (near) id = pick_exact<LT, VPL>(a, row);
+            if (near) {
+                id = pick_exact<LT, VPL>(a, row);
+            } else if (__any_sync(kFull, close)) {
+                // Every expert that can be among the chosen: those taken (the first one
+                // not chosen, too) and what is left within reach of the last slot's key.
+                int n = min(__popc(__ballot_sync(kFull, mine != 0u)), a.topk) + (more != 0u);
+                const float v = value_of(__shfl_sync(kFull, mine, a.topk - 1));
+                const float big = a.bare ? fabsf(v) : size;
+                const unsigned reach = more ? order_of(v - (abs_off + 2.0f * rel * big)) : ~0u;
+#pragma unroll
+                for (int k = 0; k < VPL; ++k) {
+                    const unsigned in = __ballot_sync(kFull, list[k] != 0u && list[k] >= reach);
+                    if ((in >> lane & 1u) && n + __popc(in & below) < 32)
+                        picked[warp][n + __popc(in & below)] =
+                            sp.base + VPL - 1 - (int)(list[k] & (VPL - 1));
+                    n += __popc(in);
+                }
+                __syncwarp();
+                id = n <= 32 ? order_exact<LT>(a, row, picked[warp], n)
+                             : pick_exact<LT, VPL>(a, row);
+            }
+            __syncwarp();
         }
-        // lane j: slot j
-        float w = 0.0f;
-        if (a.sigmoid) {
-            if (id >= 0) w = sigmoid_f(clean_logit(to_f32(row[id])));
+        // this token's slots to their lanes of the run
+        const int from = lane & ((1 << a.slots_log) - 1);
+        const int moved = __shfl_sync(kFull, id, from);
+        if (lane >> a.slots_log == in_run) {
+            run_id = from < a.topk ? moved : -1;
+            run_m = m;
+            run_sum = sum;
+        }
+        if (++in_run == per || t + 1 == a.T) {
+            const long long token = t + 1 - in_run + (lane >> a.slots_log);
+            const bool mine = lane >> a.slots_log < in_run;
+            float w = 0.0f;
+            const float z = mine && run_id >= 0 ? clean_logit(to_f32(logits[token * a.ld + run_id]))
+                                                : -INFINITY;
+            if (a.sigmoid) {
+                w = sigmoid_f(z);                                // -inf: 0
+            } else {
+                float top = run_m;
+                if (a.renorm) {                                  // shifted by the largest chosen
+                    top = z;
+                    for (int o = 1 << a.slots_log >> 1; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                }
+                w = z > -INFINITY ? expf(z - top) : 0.0f;
+            }
+            float total = a.sigmoid ? 1.0f : run_sum;
             if (a.renorm) {
-                const float total = warp_sum(w);
-                w = total > 0.0f ? w / total : 0.0f;
+                total = w;
+                for (int o = 1 << a.slots_log >> 1; o > 0; o >>= 1)
+                    total += __shfl_xor_sync(kFull, total, o);
             }
-        } else {
-            const float z = id >= 0 ? clean_logit(to_f32(row[id])) : -INFINITY;
-            const float top = a.renorm ? warp_max(z) : m;     // shifted by the largest chosen one
-            if (id >= 0) w = expf(z - top);
-            const float total = a.renorm ? warp_sum(w) : sum;
-            w = id >= 0 ? w / total : 0.0f;
+            w = total > 0.0f ? w / total : 0.0f;
+            if (mine && from < a.topk) {
+                a.weights[token * a.topk + from] = a.scale * w;
+                a.ids[token * a.topk + from] = run_id;
+            }
+            in_run = 0;
         }
-        if (lane < a.topk) {
-            a.weights[t * a.topk + lane] = a.scale * w;
-            a.ids[t * a.topk + lane] = id;
-        }
+        t = t_next;
     }
 }
 
@@ -292,102 +496,174 @@ struct RouteBwdArgs {
     long long ld;
     const int32_t* ids;
     int T, E, topk;
+    int slots;            // lanes per token: the power of two from topk up
     bool sigmoid, renorm;
     float scale;
     void* dlogits;
 };
 
-template <typename LT>
-__global__ void __launch_bounds__(kRouteWarps * 32) moe_route_bwd_kernel(const RouteBwdArgs a) {
+// A warp takes 32 / P tokens at a time, P the power of two from topk up: lane
+// P i + j holds slot j of token i.  Rows are written by the whole warp.  NV: vectors
+// of 4 columns per lane, columns 4 (32 i + lane) ..+3.
+template <typename LT, int NV, bool VEC>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+    moe_route_bwd_kernel(const __grid_constant__ RouteBwdArgs a) {
     pdl_begin();
     const int lane = threadIdx.x & 31;
+    const int P = a.slots, per = 32 / P, slot = lane % P;
     const bool dense = !a.sigmoid && !a.renorm;
-    for (long long t = (long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T;
-         t += (long long)gridDim.x * kRouteWarps) {
+    auto slots_sum = [&](float v) {
+        for (int o = P >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+        return v;
+    };
+    for (long long t0 = ((long long)blockIdx.x * kRouteWarps + (threadIdx.x >> 5)) * per; t0 < a.T;
+         t0 += (long long)gridDim.x * kRouteWarps * per) {
+        const long long t = t0 + lane / P;
+        const int tokens = (int)min((long long)per, a.T - t0);
         const LT* row = static_cast<const LT*>(a.logits) + t * a.ld;
         LT* out = static_cast<LT*>(a.dlogits) + t * a.E;
-        int id = lane < a.topk ? a.ids[t * a.topk + lane] : -1;
-        if (id >= a.E) id = -1;
-        const float g = id >= 0 ? a.scale * a.grad[t * a.topk + lane] : 0.0f;
+        int id = -1;
+        float g = 0.0f;
+        if (slot < a.topk && t < a.T) {
+            id = a.ids[t * a.topk + slot];
+            g = a.scale * a.grad[t * a.topk + slot];
+        }
+        if (id < 0 || id >= a.E) id = -1, g = 0.0f;
         const float z = id >= 0 ? clean_logit(to_f32(row[id])) : -INFINITY;
 
-        float m = 0.0f, sum = 1.0f;
+        // d: this slot's contribution to dz at its id; once: what comes off once per id
+        float d = 0.0f, once = 0.0f;
         if (dense) {
-            m = -INFINITY;
-            for (int e = lane; e < a.E; e += 32) m = fmaxf(m, clean_logit(to_f32(row[e])));
-            m = warp_max(m);
-            sum = 0.0f;
-            if (m > -INFINITY)
-                for (int e = lane; e < a.E; e += 32) sum += expf(clean_logit(to_f32(row[e])) - m);
-            sum = warp_sum(sum);
-        }
-        // d: this slot's contribution to dz at its id
-        float d = 0.0f, inner = 0.0f;
-        if (dense) {
-            const float p = z > -INFINITY ? expf(z - m) / sum : 0.0f;
-            inner = warp_sum(g * p);
-            d = p * g;                                    // - p * inner, once per id, below
-        } else if (!a.renorm) {
-            const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
-            d = z > -INFINITY ? g * e * r * r : 0.0f;     // s (1 - s)
+            for (int i = 0; i < tokens; ++i) {
+                const LT* r = static_cast<const LT*>(a.logits) + (t0 + i) * a.ld;
+                LT e[NV][4];
+                float p[NV][4];
+                float m = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) load4<LT, VEC>(r, 4 * (32 * n + lane), a.E, e[n]);
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        p[n][k] = 4 * (32 * n + lane) + k < a.E ? clean_logit(to_f32(e[n][k]))
+                                                                : -INFINITY;
+                        m = fmaxf(m, p[n][k]);
+                    }
+                m = warp_max(m);
+                if (!(m > -INFINITY)) m = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        p[n][k] = expf(p[n][k] - m);
+                        sum += p[n][k];
+                    }
+                sum = warp_sum(sum);
+                const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+                const float p_id = expf(z - m) * inv;        // of the lanes of token i
+                const float inner = __shfl_sync(kFull, slots_sum(g * p_id), i * P);
+                if (lane / P == i) d = p_id * g, once = p_id * inner;
+#pragma unroll
+                for (int n = 0; n < NV; ++n) {
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = -(p[n][k] * inv) * inner;
+                    store4<LT, VEC>(static_cast<LT*>(a.dlogits) + (t0 + i) * a.E,
+                                    4 * (32 * n + lane), a.E, v);
+                }
+            }
         } else {
-            float w, rest = 1.0f;
-            if (a.sigmoid) {
-                w = z > -INFINITY ? sigmoid_f(z) : 0.0f;
-                rest = sigmoid_f(-z);                     // 1 - s
+            const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < tokens; ++i)
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+                    store4<LT, VEC>(static_cast<LT*>(a.dlogits) + (t0 + i) * a.E,
+                                    4 * (32 * n + lane), a.E, none);
+            if (!a.renorm) {
+                const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
+                d = g * e * r * r;                        // s (1 - s); -inf: e = 0
             } else {
-                const float top = warp_max(z);
-                w = z > -INFINITY ? expf(z - top) : 0.0f;
-            }
-            const float total = warp_sum(w);
-            w = total > 0.0f ? w / total : 0.0f;
-            d = w * (g - warp_sum(g * w)) * rest;
-            if (!(z > -INFINITY)) d = 0.0f;
-        }
-        // slots with the same id: the first of them writes the sum
-        float all = 0.0f;
-        bool first = id >= 0;
-        for (int j = 0; j < a.topk; ++j) {
-            const int other = __shfl_sync(kFull, id, j);
-            const float dj = __shfl_sync(kFull, d, j);
-            if (other == id) {
-                all += dj;
-                if (j < lane) first = false;
+                float w, rest = 1.0f;
+                if (a.sigmoid) {
+                    w = sigmoid_f(z);                     // -inf: 0
+                    rest = sigmoid_f(-z);                 // 1 - s
+                } else {
+                    float top = z;
+                    for (int o = P >> 1; o > 0; o >>= 1)
+                        top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                    w = z > -INFINITY ? expf(z - top) : 0.0f;
+                }
+                const float total = slots_sum(w);
+                w = total > 0.0f ? w / total : 0.0f;
+                d = w * (g - slots_sum(g * w)) * rest;
             }
         }
-        if (dense) {
-            for (int e = lane; e < a.E; e += 32) {
-                const float ze = clean_logit(to_f32(row[e]));
-                out[e] = from_f32<LT>(ze > -INFINITY ? -(expf(ze - m) / sum) * inner : 0.0f);
+        // slots of a token with the same id add up in slot order; the first writes the sum
+        const unsigned same = __match_any_sync(kFull, id < 0 ? -1 - lane : id + lane / P * a.E);
+        float all = d;
+        if (__any_sync(kFull, __popc(same) > 1)) {
+            all = 0.0f;
+            for (int j = 0; j < 32; ++j) {
+                const float dj = __shfl_sync(kFull, d, j);
+                if (same >> j & 1u) all += dj;
             }
-            if (z > -INFINITY) all -= expf(z - m) / sum * inner;
-        } else {
-            for (int e = lane; e < a.E; e += 32) out[e] = from_f32<LT>(0.0f);
         }
         __syncwarp();
-        if (first) out[id] = from_f32<LT>(all);
+        if (id >= 0 && __ffs(same) - 1 == lane) out[id] = from_f32<LT>(all - once);
+        __syncwarp();
     }
+}
+
+template <typename LT, int VPL, bool VEC>
+int launch_route(const RouteArgs& a, int sms, cudaStream_t s) {
+    // as many CTAs as are resident at once
+    static const int per_sm = [] {
+        int n = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, moe_route_kernel<LT, VPL, VEC>,
+                                                          kRouteWarps * 32, 0) != cudaSuccess)
+            cudaGetLastError();
+        return n > 0 ? n : 4;
+    }();
+    const int per = kRouteWarps * (32 >> a.slots_log);
+    const long long want = ((long long)a.T + per - 1) / per;
+    const dim3 grid((unsigned)std::min(want, (long long)sms * per_sm)), block(kRouteWarps * 32);
+    return launch_kernel(moe_route_kernel<LT, VPL, VEC>, grid, block, 0, s, a);
+}
+
+template <typename LT, int VPL>
+int launch_route(const RouteArgs& a, bool vec, int sms, cudaStream_t s) {
+    return vec ? launch_route<LT, VPL, true>(a, sms, s) : launch_route<LT, VPL, false>(a, sms, s);
 }
 
 template <typename LT>
 int run_route(const RouteArgs& a, int sms, cudaStream_t s) {
     const int lpg = 32 / a.n_group, G = a.E / a.n_group, vpl = (G + lpg - 1) / lpg;
-    const long long want = ((long long)a.T + kRouteWarps - 1) / kRouteWarps;
-    const long long most = (long long)sms * 64;
-    const dim3 grid((unsigned)(want < most ? want : most)), block(kRouteWarps * 32);
-    if (vpl <= 2) return launch_kernel(moe_route_kernel<LT, 2>, grid, block, 0, s, a);
-    if (vpl <= 4) return launch_kernel(moe_route_kernel<LT, 4>, grid, block, 0, s, a);
-    if (vpl <= 8) return launch_kernel(moe_route_kernel<LT, 8>, grid, block, 0, s, a);
-    if (vpl <= 16) return launch_kernel(moe_route_kernel<LT, 16>, grid, block, 0, s, a);
-    return launch_kernel(moe_route_kernel<LT, 32>, grid, block, 0, s, a);
+    const bool rows = a.ld % 4 == 0 && aligned_to(a.logits, 4 * sizeof(LT));
+    const bool full = G == vpl * lpg;          // every lane holds the same number
+    if (vpl <= 2) return launch_route<LT, 2>(a, false, sms, s);
+    if (vpl <= 4) return launch_route<LT, 4>(a, rows && full && vpl == 4, sms, s);
+    if (vpl <= 8) return launch_route<LT, 8>(a, rows && full && vpl == 8, sms, s);
+    if (vpl <= 16) return launch_route<LT, 16>(a, rows && full && vpl == 16, sms, s);
+    return launch_route<LT, 32>(a, rows && full && vpl == 32, sms, s);
+}
+
+template <typename LT, int NV>
+int launch_route_bwd(const RouteBwdArgs& a, bool vec, int sms, cudaStream_t s) {
+    const int per = kRouteWarps * (32 / a.slots);
+    const long long want = ((long long)a.T + per - 1) / per;
+    const dim3 grid((unsigned)std::min(want, (long long)sms * 64)), block(kRouteWarps * 32);
+    return vec ? launch_kernel(moe_route_bwd_kernel<LT, NV, true>, grid, block, 0, s, a)
+               : launch_kernel(moe_route_bwd_kernel<LT, NV, false>, grid, block, 0, s, a);
 }
 
 template <typename LT>
 int run_route_bwd(const RouteBwdArgs& a, int sms, cudaStream_t s) {
-    const long long want = ((long long)a.T + kRouteWarps - 1) / kRouteWarps;
-    const long long most = (long long)sms * 64;
-    const dim3 grid((unsigned)(want < most ? want : most)), block(kRouteWarps * 32);
-    return launch_kernel(moe_route_bwd_kernel<LT>, grid, block, 0, s, a);
+    const bool vec = a.E % 4 == 0 && a.ld % 4 == 0 && aligned_to(a.logits, 4 * sizeof(LT)) &&
+                     aligned_to(a.dlogits, 4 * sizeof(LT));
+    if (a.E <= 128) return launch_route_bwd<LT, 1>(a, vec, sms, s);
+    if (a.E <= 256) return launch_route_bwd<LT, 2>(a, vec, sms, s);
+    if (a.E <= 512) return launch_route_bwd<LT, 4>(a, vec, sms, s);
+    return launch_route_bwd<LT, 8>(a, vec, sms, s);
 }
 
 }  // namespace
@@ -417,9 +693,15 @@ extern "C" int ferret_moe_route(const void* logits, long long ld, int dtype, con
     if (rc != FERRET_OK) return rc;
     // every group open: the groups decide nothing
     if (topk_group == n_group) n_group = topk_group = 1;
+    int lpg_log = 5, slots_log = 0;
+    while (32 >> lpg_log < n_group) --lpg_log;
+    while (1 << slots_log < topk) ++slots_log;
+    // shorter runs while there are too few of them for every SM's 24 warps
+    while (slots_log < 5 && T >> (5 - slots_log) < info->num_sms * 24) ++slots_log;
     const RouteArgs a{logits, ld, bias, token_mask, T, E, topk, n_group, topk_group, group_top,
+                      lpg_log, slots_log,
                       (flags & FERRET_ROUTE_SIGMOID) != 0, (flags & FERRET_ROUTE_RENORM) != 0,
-                      scale, weights, ids};
+                      !bias && (n_group == 1 || group_top == 1), scale, weights, ids};
     const cudaStream_t s = as_stream(stream);
     switch (dtype) {
         case FERRET_BF16: return run_route<__nv_bfloat16>(a, info->num_sms, s);
@@ -444,7 +726,9 @@ extern "C" int ferret_moe_route_backward(const float* grad_weights, const void* 
     DeviceInfo* info = nullptr;
     int rc = current_device(&info);
     if (rc != FERRET_OK) return rc;
-    const RouteBwdArgs a{grad_weights, logits, ld, ids, T, E, topk,
+    int slots = 1;
+    while (slots < topk) slots *= 2;
+    const RouteBwdArgs a{grad_weights, logits, ld, ids, T, E, topk, slots,
                          (flags & FERRET_ROUTE_SIGMOID) != 0, (flags & FERRET_ROUTE_RENORM) != 0,
                          scale, grad_logits};
     const cudaStream_t s = as_stream(stream);

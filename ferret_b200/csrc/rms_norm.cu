@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const NormArgs a
         ss = warp_sum(lane < (tpr >> 5) ? warp_sums[odd][lane] : 0.0f);
         finish_row<T, NV, true>(a, row, tid, true, v, ss);
     }
-    // a wait ran out: let the copies in flight land before the CTA leaves
+    // a wait ran out: the copies in flight land before the CTA leaves (slots
+    // that hold no further row end this wait by its time limit)
     if (abort_flag && tid == 0)
         for (int i = 0; i < stages; ++i, pos.advance(stages))
             mbar_wait(smem_addr(&full[pos.slot]), pos.phase, &abort_flag, ctl, 22, false);

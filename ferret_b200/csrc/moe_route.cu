@@ -8,7 +8,7 @@
 //            keys have the largest sum stay open
 //   choice   the topk open experts with the largest keys, largest first, the
 //            lower id first among equals
-//   weights  scale * s[id], divided by their sum when renormalized
+//   weights  scale * s[id], divided by the sum of the chosen s when renormalized
 // A logit of -inf or NaN closes its expert (score 0); slots with no open
 // expert left, and every slot of a token outside the mask, get id -1 and
 // weight 0, which the permutation and the combine skip.
@@ -16,11 +16,11 @@
 // Which of two keys is larger decides an integer, so the order has to be that
 // of the exact keys.  The selection runs on approximate keys (fast fp32
 // scores, the low bits of a key's integer image traded for the expert's place in
-// its lane) and looks at the gap between each chosen key and the next: where
-// a gap is below the bound on the approximation and the two experts are not
-// equal by their inputs, the token takes a second selection with keys in fp64
-// (under one token in a hundred).  Without a bias the score is monotone in z,
-// and z itself is the key.
+// its lane) and looks at the gap between each chosen key and the next: where a gap is
+// below the bound on the approximation, and the two experts are not both chosen
+// and equal by their inputs, the experts in reach are ordered by keys in fp64
+// (under one token in a hundred of fp32 logits).  Without a bias the score is
+// monotone in z, and z itself is the key.
 //
 // HBM-bound at large T (the logits are read once), latency-bound at small T; in
 // between the instructions of the selection bound it.  One warp per token, the
@@ -57,10 +57,10 @@ struct RouteArgs {
     int32_t* ids;
 };
 
-// sigmoid(z) without cancellation or overflow on either side.
-__device__ __forceinline__ float sigmoid_f(float z) {
-    const float e = expf(-fabsf(z));
-    return (z >= 0.0f ? 1.0f : e) / (1.0f + e);
+// sigmoid(z) / e^shift, shift <= 0: with the shift of the largest of several z a
+// quotient of sigmoids does not underflow.
+__device__ __forceinline__ float sigmoid_over(float z, float shift) {
+    return expf(fminf(z, 0.0f) - shift) / (1.0f + expf(-fabsf(z)));
 }
 __device__ __forceinline__ double sigmoid_d(double z) {
     const double e = exp(-fabs(z));
@@ -300,8 +300,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
     // A key's integer image with its place in the lane, 0 for a closed expert
     // (bias 0 turns -0 into +0; the largest finite value stands for +inf).
     auto image = [&](float v, int k, bool open) {
-        v = fminf(v, 3.402823466e38f);
-        const unsigned o = (order_of(v) & ~(unsigned)(VPL - 1)) | (unsigned)(VPL - 1 - k);
+        const unsigned o = (order_of(fminf(v, 3.402823466e38f)) & ~(unsigned)(VPL - 1)) | (unsigned)(VPL - 1 - k);
         return open && v > -INFINITY && (VEC || k < sp.n) ? o : 0u;
     };
     int in_run = 0, run_id = -1;
@@ -408,8 +407,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
                     const float v = value_of(mine), w = value_of(after);
                     const float big = a.bare ? fmaxf(fabsf(v), fabsf(w)) : size;
                     if (v - w <= abs_off + rel * big) {
+                        // Two chosen experts equal by their inputs are in order.  At the
+                        // border a third one, in reach but not looked at, may differ.
                         const int other = picked[warp][lane + 1];
-                        close = clean_logit(to_f32(row[id])) != clean_logit(to_f32(row[other])) ||
+                        close = lane == a.topk - 1 ||
+                                clean_logit(to_f32(row[id])) != clean_logit(to_f32(row[other])) ||
                                 (a.bias && a.bias[id] != a.bias[other]);
                     }
                 }
@@ -451,17 +453,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
             float w = 0.0f;
             const float z = mine && run_id >= 0 ? clean_logit(to_f32(logits[token * a.ld + run_id]))
                                                 : -INFINITY;
-            if (a.sigmoid) {
-                w = sigmoid_f(z);                                // -inf: 0
-            } else {
-                float top = run_m;
-                if (a.renorm) {                                  // shifted by the largest chosen
-                    top = z;
-                    for (int o = 1 << a.slots_log >> 1; o > 0; o >>= 1)
-                        top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-                }
-                w = z > -INFINITY ? expf(z - top) : 0.0f;
+            float top = a.sigmoid ? 0.0f : run_m;
+            if (a.renorm) {                                  // shifted by the largest chosen
+                top = z;
+                for (int o = 1 << a.slots_log >> 1; o > 0; o >>= 1)
+                    top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
             }
+            if (z > -INFINITY) w = a.sigmoid ? sigmoid_over(z, fminf(top, 0.0f)) : expf(z - top);
             float total = a.sigmoid ? 1.0f : run_sum;
             if (a.renorm) {
                 total = w;
@@ -583,16 +581,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32)
                 const float e = expf(-fabsf(z)), r = 1.0f / (1.0f + e);
                 d = g * e * r * r;                        // s (1 - s); -inf: e = 0
             } else {
-                float w, rest = 1.0f;
-                if (a.sigmoid) {
-                    w = sigmoid_f(z);                     // -inf: 0
-                    rest = sigmoid_f(-z);                 // 1 - s
-                } else {
-                    float top = z;
-                    for (int o = P >> 1; o > 0; o >>= 1)
-                        top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-                    w = z > -INFINITY ? expf(z - top) : 0.0f;
-                }
+                float top = z, w = 0.0f;
+                for (int o = P >> 1; o > 0; o >>= 1)
+                    top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+                if (z > -INFINITY)
+                    w = a.sigmoid ? sigmoid_over(z, fminf(top, 0.0f)) : expf(z - top);
+                const float rest = a.sigmoid ? sigmoid_over(-z, 0.0f) : 1.0f;      // 1 - s
                 const float total = slots_sum(w);
                 w = total > 0.0f ? w / total : 0.0f;
                 d = w * (g - slots_sum(g * w)) * rest;

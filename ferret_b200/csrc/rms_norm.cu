@@ -282,7 +282,7 @@ template <typename T, int NV>
 int launch_ring(const NormArgs& a, int ctas_per_sm, int stages, size_t smem, const DeviceInfo* info,
                 cudaStream_t s) {
     auto kern = add_rms_norm_ring_kernel<T, NV>;
-    if (smem > 48 * 1024 &&
+    if (smem > 40 * 1024 &&           // 48 KB less the static arrays need no opt-in
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
             cudaSuccess) {
         cudaGetLastError();

@@ -22,6 +22,26 @@ of the baselines it replaces:
   moe_wna16_marlin_gemm + SiLU
   (baseline_marlin.py:140-168).
 
+and, for the operators around the expert layer (no reference counterpart):
+
+* ``ferret_moe::add_rms_norm(Tensor x, Tensor residual, Tensor weight, float
+  eps=1e-6) -> (Tensor, Tensor)`` and ``add_rms_norm_fp8(..., bool
+  use_ue8m0=False) -> (Tensor, Tensor, Tensor, Tensor)``;
+* ``ferret_moe::moe_route(Tensor logits, int topk, ...) -> (Tensor weights,
+  Tensor ids)`` and ``moe_balance_loss(Tensor logits, Tensor topk_ids, float
+  coef, ...) -> (Tensor loss, Tensor counts, Tensor prob_sums, Tensor
+  n_tokens)``, both differentiable in the logits (weights and loss; the other
+  outputs carry no gradient);
+* ``ferret_moe::int4_linear(Tensor x, Tensor w, Tensor w_scale, Tensor?
+  w_zero=None, Tensor? bias=None) -> Tensor``.
+
+A differentiable call is refused while its stream is being captured into a CUDA
+graph, forward and backward: a captured backward pass that meets gradient
+accumulators of an eager graph on another stream breaks the capture beyond
+repair.  Captured training steps call ``ops.moe_route``,
+``ops.moe_route_backward``, ``ops.moe_balance_loss`` and
+``ops.moe_balance_loss_backward``, which record no autograd graph.
+
 Every operator runs the CUDA library (CUDA tensors only); importing this
 module registers them.
 """
@@ -74,3 +94,96 @@ _LIB.impl("fp8_grouped_gemm_nt_contiguous", _fp8_gemm, "CUDA")
 _LIB.impl("per_token_cast_to_fp8", _quant, "CUDA")
 _LIB.impl("moe_align_block_size", _align, "CUDA")
 _LIB.impl("int4_moe_w13", _int4, "CUDA")
+
+
+# ----------------------------------------------------- around the expert layer
+
+_LIB.define("add_rms_norm(Tensor x, Tensor residual, Tensor weight, float eps=1e-6) "
+            "-> (Tensor, Tensor)")
+_LIB.define("add_rms_norm_fp8(Tensor x, Tensor residual, Tensor weight, float eps=1e-6, "
+            "bool use_ue8m0=False) -> (Tensor, Tensor, Tensor, Tensor)")
+_LIB.define("moe_route(Tensor logits, int topk, str scoring='softmax', Tensor? bias=None, "
+            "int n_group=1, int topk_group=1, int group_top=2, bool renormalize=False, "
+            "float scale=1.0, Tensor? token_mask=None) -> (Tensor, Tensor)")
+_LIB.define("moe_balance_loss(Tensor logits, Tensor topk_ids, float coef, str scoring='softmax', "
+            "Tensor? token_mask=None) -> (Tensor, Tensor, Tensor, Tensor)")
+_LIB.define("int4_linear(Tensor x, Tensor w, Tensor w_scale, Tensor? w_zero=None, "
+            "Tensor? bias=None) -> Tensor")
+
+
+def _norm(x, residual, weight, eps=1e-6):
+    return ops.add_rms_norm(x, weight, residual, eps)[:2]
+
+
+def _norm_fp8(x, residual, weight, eps=1e-6, use_ue8m0=False):
+    return ops.add_rms_norm(x, weight, residual, eps, quant=True, use_ue8m0=use_ue8m0)
+
+
+def _route(logits, topk, scoring="softmax", bias=None, n_group=1, topk_group=1, group_top=2,
+           renormalize=False, scale=1.0, token_mask=None):
+    return ops.moe_route(logits, topk, scoring=scoring, bias=bias, n_group=n_group,
+                         topk_group=topk_group, group_top=group_top, renormalize=renormalize,
+                         scale=scale, token_mask=token_mask)
+
+
+def _balance(logits, topk_ids, coef, scoring="softmax", token_mask=None):
+    return ops.moe_balance_loss(logits, topk_ids, coef, scoring=scoring, token_mask=token_mask)
+
+
+def _int4_linear(x, w, w_scale, w_zero=None, bias=None):
+    return ops.int4_linear(x, w, w_scale, w_zero=w_zero, bias=bias)
+
+
+def _not_captured(name):
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"torch.ops.ferret_moe.{name} does not record gradients inside a CUDA "
+                           f"graph capture: capture ops.{name} and ops.{name}_backward instead")
+
+
+def _route_setup(ctx, inputs, output):
+    _not_captured("moe_route")
+    logits, _, scoring, _, _, _, _, renormalize, scale, _ = inputs
+    _, ids = output
+    ctx.mark_non_differentiable(ids)
+    ctx.save_for_backward(logits, ids)
+    ctx.form = dict(scoring=scoring, renormalize=renormalize, scale=scale)
+
+
+def _route_backward(ctx, grad_weights, _):
+    _not_captured("moe_route")
+    logits, ids = ctx.saved_tensors
+    grad = None
+    if grad_weights is not None:
+        grad = ops.moe_route_backward(grad_weights.contiguous(), logits, ids, **ctx.form)
+    return grad, *[None] * 9
+
+
+def _balance_setup(ctx, inputs, output):
+    _not_captured("moe_balance_loss")
+    logits, topk_ids, coef, scoring, token_mask = inputs
+    _, counts, prob_sums, n_tokens = output
+    ctx.mark_non_differentiable(counts, prob_sums, n_tokens)
+    ctx.save_for_backward(logits, counts, n_tokens, token_mask)
+    ctx.form = (topk_ids.shape[1], coef, scoring)
+
+
+def _balance_backward(ctx, grad_loss, *_):
+    _not_captured("moe_balance_loss")
+    logits, counts, n_tokens, token_mask = ctx.saved_tensors
+    topk, coef, scoring = ctx.form
+    grad = None
+    if grad_loss is not None:
+        grad = ops.moe_balance_loss_backward(grad_loss.contiguous(), logits, counts, n_tokens, topk,
+                                             coef, scoring=scoring, token_mask=token_mask)
+    return grad, None, None, None, None
+
+
+_LIB.impl("add_rms_norm", _norm, "CUDA")
+_LIB.impl("add_rms_norm_fp8", _norm_fp8, "CUDA")
+_LIB.impl("moe_route", _route, "CUDA")
+_LIB.impl("moe_balance_loss", _balance, "CUDA")
+_LIB.impl("int4_linear", _int4_linear, "CUDA")
+torch.library.register_autograd("ferret_moe::moe_route", _route_backward,
+                                setup_context=_route_setup, lib=_LIB)
+torch.library.register_autograd("ferret_moe::moe_balance_loss", _balance_backward,
+                                setup_context=_balance_setup, lib=_LIB)

@@ -371,7 +371,7 @@ FERRET_API int ferret_add_rms_norm(const void* x, long long ldx, const void* res
  * exact keys: keys closer than their fp32 rounding are compared in fp64.
  * ids int32 [T, topk]; weights f32 [T, topk] = scale * score (without the
  * bias), divided by the sum of the token's chosen scores with
- * FERRET_ROUTE_RENORM (0 if that sum is 0).
+ * FERRET_ROUTE_RENORM (also where the scores themselves underflow).
  * A logit of -inf or NaN, or a bias of -inf or NaN, closes its expert; +inf
  * counts as the largest finite value.  Slots without an open expert, and all
  * slots of a token whose token_mask byte (uint8 [T] or NULL) is 0, have id -1

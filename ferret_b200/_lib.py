@@ -105,6 +105,26 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+_HOST = None
+
+
+def host():
+    """The extension module ``ferret_b200._host`` (argument checks, outputs and the
+    C-ABI call of the operators around the expert GEMMs)."""
+    global _HOST
+    if _HOST is None:
+        lib()
+        try:
+            from . import _host
+        except ImportError as e:
+            raise ImportError(
+                f"ferret_b200 host module not usable ({e}); build it with "
+                "`python -m ferret_b200.build`") from e
+        _host.set_check(check)
+        _HOST = _host
+    return _HOST
+
+
 def strerror(code: int) -> str:
     try:
         return lib().ferret_strerror(code).decode()

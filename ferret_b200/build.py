@@ -6,7 +6,9 @@ Each ``csrc/*.cu`` is compiled by nvcc into ``_build/`` (in parallel) and the
 objects are linked into one shared library with the CUDA runtime linked
 statically, so the library loads on machines without a GPU driver (the
 driver-API entry point the TMA descriptors need is resolved at run time
-through the runtime).  ``kernel_result.cu`` becomes the benchmark binary
+through the runtime).  ``csrc/host.cpp`` becomes the extension module
+``ferret_b200/_host.so`` (g++ against the installed torch, linked to that
+library next to it).  ``kernel_result.cu`` becomes the benchmark binary
 ``ferret_b200/ferret_kernel_result`` linked against that library.
 """
 from __future__ import annotations
@@ -17,12 +19,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libferret_moe.so")
 BIN = os.path.join(HERE, "ferret_kernel_result")
+HOST = os.path.join(HERE, "_host.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -58,7 +62,7 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
     deps = _deps()
-    if not force and not _stale(LIB, deps + [__file__]) and not _stale(BIN, deps + [__file__]):
+    if not force and not any(_stale(t, deps + [__file__]) for t in (LIB, BIN, HOST)):
         return LIB
     cc = nvcc()
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
@@ -89,6 +93,7 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
     build_kernel_result(cc, verbose)
+    build_host(verbose)
     return LIB
 
 
@@ -104,6 +109,30 @@ def build_kernel_result(cc: str, verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"kernel_result build failed:\n{r.stdout}\n{r.stderr}")
     return BIN
+
+
+def build_host(verbose: bool = False) -> str:
+    """The extension module of the operators' host side, linked against the
+    library next to it and the installed torch."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    tmp = HOST + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", os.path.join(root, "include"),
+           "-I", os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I", sysconfig.get_paths()["include"], "-I", os.path.join(cuda, "include"),
+           os.path.join(CSRC, "host.cpp"), "-o", tmp, "-L", HERE, "-lferret_moe",
+           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda",
+           "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"host module build failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST)
+    return HOST
 
 
 def main():

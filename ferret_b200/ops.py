@@ -29,9 +29,8 @@ import ctypes
 
 import torch
 
-from ._lib import (FERRET_BF16, FERRET_FP16, FERRET_FP32, FERRET_PREFILL_PAIRS,
-                   FERRET_ROUTE_RENORM, FERRET_ROUTE_SIGMOID, FERRET_SILU_MUL, FERRET_TILE_SHIFT,
-                   FERRET_UE8M0_SCALES, check, lib)
+from ._lib import (FERRET_PREFILL_PAIRS, FERRET_SILU_MUL, FERRET_TILE_SHIFT, FERRET_UE8M0_SCALES,
+                   check, host, lib)
 
 
 def _ptr(t: torch.Tensor | None):
@@ -403,58 +402,9 @@ def moe_wna16_w13(hidden: torch.Tensor, weights: Int4W13Weights, topk_ids: torch
     return out
 
 
-# ------------------------------------------- around the expert layer: helpers
-
-_DTYPES = {torch.bfloat16: FERRET_BF16, torch.float16: FERRET_FP16, torch.float32: FERRET_FP32}
-_raw_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _call(name: str, dev: int, args) -> None:
-    """The library call ``name`` on the tensors' device and that device's current stream."""
-    fn = getattr(lib(), name)
-    if dev == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _raw_stream(dev))
-    if rc:
-        check(rc, name)
-
-
-def _cuda(t: torch.Tensor, name: str) -> int:
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{name} must be a CUDA tensor")
-    return dev
-
-
-def _like(t: torch.Tensor | None, name: str, dev: int, dtype, shape) -> int | None:
-    """Address of a contiguous tensor of that device, type and shape (None passes)."""
-    if t is None:
-        return None
-    if t.get_device() != dev:
-        raise ValueError(f"{name} must be on the device of the first argument")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
-
-
-def _rows(t: torch.Tensor, name: str) -> int:
-    """Row stride of a matrix whose rows are contiguous and do not overlap."""
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
-    T, K = t.shape
-    if T >= 2**31 or K >= 2**31:
-        raise ValueError(f"{name} is too large: {tuple(t.shape)}")
-    ld, inner = t.stride()
-    if (inner != 1 and K > 1) or (ld < K and T > 1):
-        raise ValueError(f"{name} must have contiguous rows that do not overlap")
-    return ld if T > 1 else K
-
+# Around the expert layer: the functions below hand their arguments to the extension
+# module, which checks them, allocates the outputs and makes the C-ABI call on
+# the tensors' device and that device's current stream.
 
 # --------------------------------------------------------- norm with FP8 rows
 
@@ -470,54 +420,10 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     rounded s) None without a residual, q and scale None without ``quant``.
     Pass ``residual_out`` to have it written there; it may be ``residual`` or
     ``x`` itself.  With ``quant`` K must be a multiple of 128; K <= 32768."""
-    dev = _cuda(x, "x")
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
-    ldx = _rows(x, "x")
-    T, K = x.shape
-    wdt = torch.float32 if weight.dtype == torch.float32 else x.dtype
-    wp = _like(weight, "weight", dev, wdt, (K,))
-    ldr, rp = 0, None
-    if residual is not None:
-        if residual.get_device() != dev or residual.dtype != x.dtype or residual.shape != x.shape:
-            raise ValueError("residual must have the device, type and shape of x")
-        ldr, rp = _rows(residual, "residual"), residual.data_ptr()
-        if residual_out is None:
-            residual_out = torch.empty((T, K), dtype=x.dtype, device=x.device)
-    elif residual_out is not None:
-        raise ValueError("residual_out needs a residual")
-    rop = _like(residual_out, "residual_out", dev, x.dtype, (T, K))
-    y = torch.empty((T, K), dtype=x.dtype, device=x.device) if normed else None
-    q = s = None
-    if quant:
-        if K % 128:
-            raise ValueError("K must be a multiple of 128 for FP8 rows")
-        q = torch.empty((T, K), dtype=torch.float8_e4m3fn, device=x.device)
-        s = torch.empty((T, K // 128), dtype=torch.float32, device=x.device)
-    elif not normed:
-        raise ValueError("nothing to compute: normed and quant are both off")
-    _call("ferret_add_rms_norm", dev,
-          (x.data_ptr(), ldx, rp, ldr, wp, _DTYPES[wdt], _DTYPES[x.dtype], T, K, eps,
-           y.data_ptr() if normed else None, rop, q.data_ptr() if quant else None,
-           s.data_ptr() if quant else None, FERRET_UE8M0_SCALES if use_ue8m0 else 0))
-    return y, residual_out, q, s
+    return host().add_rms_norm(x, weight, residual, eps, quant, use_ue8m0, normed, residual_out)
 
 
 # -------------------------------------------------------- routing and balance
-
-def _scoring_flags(scoring: str, renormalize: bool = False) -> int:
-    if scoring not in ("softmax", "sigmoid"):
-        raise ValueError(f"scoring must be 'softmax' or 'sigmoid', got {scoring!r}")
-    return ((FERRET_ROUTE_SIGMOID if scoring == "sigmoid" else 0)
-            | (FERRET_ROUTE_RENORM if renormalize else 0))
-
-
-def _logits(logits: torch.Tensor):
-    dev = _cuda(logits, "logits")
-    if logits.dtype not in _DTYPES:
-        raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    return dev, _rows(logits, "logits"), _DTYPES[logits.dtype], *logits.shape
-
 
 def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax",
               bias: torch.Tensor | None = None, n_group: int = 1, topk_group: int = 1,
@@ -536,16 +442,8 @@ def moe_route(logits: torch.Tensor, topk: int, *, scoring: str = "softmax",
     slots without an open expert and tokens outside ``token_mask`` (bool [T])
     get id -1, weight 0.  Limits: E <= 1024, topk <= 32.
     """
-    dev, ld, dt, T, E = _logits(logits)
-    flags = _scoring_flags(scoring, renormalize)
-    bp = _like(bias, "bias", dev, torch.float32, (E,))
-    mp = _like(token_mask, "token_mask", dev, torch.bool, (T,))
-    weights = torch.empty((T, topk), dtype=torch.float32, device=logits.device)
-    ids = torch.empty((T, topk), dtype=torch.int32, device=logits.device)
-    _call("ferret_moe_route", dev,
-          (logits.data_ptr(), ld, dt, bp, mp, T, E, topk, n_group, topk_group, group_top, scale,
-           flags, weights.data_ptr(), ids.data_ptr()))
-    return weights, ids
+    return host().moe_route(logits, topk, scoring, bias, n_group, topk_group, group_top,
+                            renormalize, scale, token_mask)
 
 
 def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: torch.Tensor, *,
@@ -553,17 +451,7 @@ def moe_route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, ids: to
                        scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``moe_route``'s weights with respect to the logits, in the
     logits' type, [T, E] (ids, scoring, renormalize and scale as there)."""
-    dev, ld, dt, T, E = _logits(logits)
-    flags = _scoring_flags(scoring, renormalize)
-    if ids.dim() != 2:
-        raise ValueError(f"ids must be 2-D, got shape {tuple(ids.shape)}")
-    topk = ids.shape[1]
-    ip = _like(ids, "ids", dev, torch.int32, (T, topk))
-    gp = _like(grad_weights, "grad_weights", dev, torch.float32, (T, topk))
-    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    _call("ferret_moe_route_backward", dev,
-          (gp, logits.data_ptr(), ld, dt, ip, T, E, topk, scale, flags, out.data_ptr()))
-    return out
+    return host().moe_route_backward(grad_weights, logits, ids, scoring, renormalize, scale)
 
 
 def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, coef: float, *,
@@ -576,23 +464,7 @@ def moe_balance_loss(logits: torch.Tensor, topk_ids: torch.Tensor, coef: float, 
     tokens' probabilities (softmax, or sigmoids divided by their sum).  Ids
     outside [0, E) are not counted.  ``counts`` is what
     ``ep.balanced_placement`` takes.  Repeatable bit for bit."""
-    dev, ld, dt, T, E = _logits(logits)
-    flags = _scoring_flags(scoring)
-    if topk_ids.dim() != 2:
-        raise ValueError(f"topk_ids must be 2-D, got shape {tuple(topk_ids.shape)}")
-    topk = topk_ids.shape[1]
-    ip = _like(topk_ids, "topk_ids", dev, torch.int32, (T, topk))
-    mp = _like(token_mask, "token_mask", dev, torch.bool, (T,))
-    loss = torch.empty((), dtype=torch.float32, device=logits.device)
-    counts = torch.empty(E, dtype=torch.int32, device=logits.device)
-    sums = torch.empty(E, dtype=torch.float32, device=logits.device)
-    live = torch.empty(1, dtype=torch.int32, device=logits.device)
-    ws_bytes = lib().ferret_moe_balance_loss_workspace_size(T, E)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=logits.device)
-    _call("ferret_moe_balance_loss", dev,
-          (logits.data_ptr(), ld, dt, ip, mp, T, E, topk, coef, flags, loss.data_ptr(),
-           counts.data_ptr(), sums.data_ptr(), live.data_ptr(), ws.data_ptr(), ws_bytes))
-    return loss, counts, sums, live
+    return host().moe_balance_loss(logits, topk_ids, coef, scoring, token_mask)
 
 
 def moe_balance_loss_backward(grad_loss: torch.Tensor, logits: torch.Tensor, counts: torch.Tensor,
@@ -602,16 +474,8 @@ def moe_balance_loss_backward(grad_loss: torch.Tensor, logits: torch.Tensor, cou
     """Gradient of ``moe_balance_loss`` with respect to the logits, in their type,
     [T, E].  grad_loss: f32 [] on the device; counts and n_tokens from the
     forward call (constants of the gradient), or both summed over ranks."""
-    dev, ld, dt, T, E = _logits(logits)
-    flags = _scoring_flags(scoring)
-    gp = _like(grad_loss, "grad_loss", dev, torch.float32, ())
-    cp = _like(counts, "counts", dev, torch.int32, (E,))
-    np_ = _like(n_tokens, "n_tokens", dev, torch.int32, (1,))
-    mp = _like(token_mask, "token_mask", dev, torch.bool, (T,))
-    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
-    _call("ferret_moe_balance_loss_backward", dev,
-          (gp, logits.data_ptr(), ld, dt, cp, np_, mp, T, E, topk, coef, flags, out.data_ptr()))
-    return out
+    return host().moe_balance_loss_backward(grad_loss, logits, counts, n_tokens, topk, coef,
+                                            scoring, token_mask)
 
 
 # ---------------------------------------------------------- dense INT4 W4A16
@@ -628,26 +492,7 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     elements).  Scales are applied in fp32 to the groups' fp32 sums.  Every 32
     tokens read the weights once: the decode form; large batches go through
     ``moe_wna16_w13`` or a dequantized GEMM."""
-    dev = _cuda(x, "x")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"x must be bf16 or fp16, got {x.dtype}")
-    ldx = _rows(x, "x")
-    T, K = x.shape
-    if w.dim() != 2 or w_scale.dim() != 2 or w.shape[0] * 8 != K:
-        raise ValueError(f"w must be [K/8, N] with K = {K}, w_scale [K/g, N]")
-    N, groups = w.shape[1], w_scale.shape[0]
-    if groups == 0 or K % groups:
-        raise ValueError(f"w_scale's {groups} rows must divide K = {K}")
-    wp = _like(w, "w", dev, torch.int32, w.shape)
-    sp = _like(w_scale, "w_scale", dev, x.dtype, (groups, N))
-    zp = _like(w_zero, "w_zero", dev, torch.int32, (groups, N // 8))
-    bp = _like(bias, "bias", dev, x.dtype, (N,))
-    if out is None:
-        out = torch.empty((T, N), dtype=x.dtype, device=x.device)
-    op = _like(out, "out", dev, x.dtype, (T, N))
-    _call("ferret_int4_linear", dev, (x.data_ptr(), ldx, wp, sp, zp, bp, _DTYPES[x.dtype], T, K, N,
-                                      K // groups, op))
-    return out
+    return host().int4_linear(x, w, w_scale, w_zero, bias, out)
 
 
 # ------------------------------------------------------------ the whole layer
@@ -655,18 +500,21 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
 def fp8_gather_rows(q: torch.Tensor, q_scale: torch.Tensor, rows: torch.Tensor, div: int = 1):
     """Rows rows[r] // div of quantized rows (e4m3 [S, K], f32 [S, K/128]) ->
     (e4m3 [R, K], f32 [R, K/128]); a negative entry gives a zero row."""
-    dev = _cuda(q, "q")
-    if q.dim() != 2 or rows.dim() != 1:
-        raise ValueError("q must be 2-D and rows 1-D")
+    _need(q, torch.float8_e4m3fn, "q", 2)
+    _need(q_scale, torch.float32, "q_scale", 2)
+    _need(rows, torch.int32, "rows", 1)
     S, K = q.shape
     R = rows.shape[0]
-    qp = _like(q, "q", dev, torch.float8_e4m3fn, (S, K))
-    sp = _like(q_scale, "q_scale", dev, torch.float32, (S, K // 128))
-    rp = _like(rows, "rows", dev, torch.int32, (R,))
-    out = torch.empty((R, K), dtype=q.dtype, device=q.device)
-    out_s = torch.empty((R, K // 128), dtype=torch.float32, device=q.device)
-    _call("ferret_fp8_gather_rows", dev,
-          (qp, sp, S, rp, div, R, K, out.data_ptr(), out_s.data_ptr()))
+    if q_scale.shape != (S, K // 128):
+        raise ValueError(f"q_scale must be [{S}, {K // 128}], got {list(q_scale.shape)}")
+    if q_scale.device != q.device or rows.device != q.device:
+        raise ValueError("q, q_scale and rows must be on one device")
+    out = torch.empty(R, K, dtype=q.dtype, device=q.device)
+    out_s = torch.empty(R, K // 128, dtype=torch.float32, device=q.device)
+    with torch.cuda.device(q.device):
+        check(lib().ferret_fp8_gather_rows(_ptr(q), _ptr(q_scale), S, _ptr(rows), div, R, K,
+                                           _ptr(out), _ptr(out_s), _stream()),
+              "ferret_fp8_gather_rows")
     return out, out_s
 
 
@@ -682,7 +530,6 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
     arguments.  Returns (out bf16 [T, H], residual_out, ids, logits): out is the
     layer's contribution, still to be added to residual_out (x itself without a
     residual), and logits with ids are what ``moe_balance_loss`` takes."""
-    dev = _cuda(x, "x")
     _need(x, torch.bfloat16, "x", 2)
     _need(gate_weight, torch.bfloat16, "gate_weight", 2)
     T, H = x.shape
@@ -693,9 +540,9 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
         raise ValueError("W2 must be [E, H, I] with I = W13.shape[1] / 2")
     for name, t in (("gate_weight", gate_weight), ("W13", W13), ("W13_scale", W13_scale),
                     ("W2", W2), ("W2_scale", W2_scale)):
-        if t.get_device() != dev:
+        if t.device != x.device:
             raise ValueError(f"{name} must be on the device of x")
-    with torch.cuda.device(dev):
+    with torch.cuda.device(x.device):
         y, res, q, s = add_rms_norm(x, norm_weight, residual, eps, quant=True)
         logits = torch.mm(y, gate_weight.t(), out_dtype=torch.float32)
         weights, ids = moe_route(logits, topk, **routing)

@@ -44,9 +44,10 @@ struct BalanceArgs {
     const uint8_t* mask;
     int T, E, topk;
     bool sigmoid;
-    float* part_sums;     // [ctas, E]
-    int32_t* part_counts; // [ctas, E]
+    float* part_sums;     // [ctas, stride]: stride is E, rounded up to whole vectors
+    int32_t* part_counts; // [ctas, stride]
     int32_t* part_live;   // [ctas]
+    int stride;
 };
 
 // A row's pieces as loaded: vector i of a lane holds columns 4 (LPT i + lane) ..+3.
@@ -174,46 +175,54 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceA
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < kBalWarps; ++w) s += sums[w][e];
-        a.part_sums[(long long)blockIdx.x * a.E + e] = s;
-        a.part_counts[(long long)blockIdx.x * a.E + e] = counts[e];
+        a.part_sums[(long long)blockIdx.x * a.stride + e] = s;
+        a.part_counts[(long long)blockIdx.x * a.stride + e] = counts[e];
     }
     if (threadIdx.x == 0) a.part_live[blockIdx.x] = live;
 }
 
 // Adds the partial tables' rows in a fixed order and forms the loss.  A CTA
-// takes 128 columns, 4 per lane; warp w adds rows w, w + 32, ...
+// takes 128 columns, 4 adjacent ones per lane; warp w adds rows w, w + 32, ..., four of
+// them in flight at a time.
 constexpr int kJoinThreads = 1024;
 constexpr int kJoinCols = 128;
+constexpr int kJoinAhead = 4;
 
 __global__ void __launch_bounds__(kJoinThreads)
     moe_balance_join_kernel(const float* part_sums, const int32_t* part_counts,
-                            const int32_t* part_live, int ctas, int E, int topk, float coef,
-                            float* loss, int32_t* counts, float* prob_sums, int32_t* n_tokens) {
+                            const int32_t* part_live, int ctas, int stride, int E, int topk,
+                            float coef, float* loss, int32_t* counts, float* prob_sums,
+                            int32_t* n_tokens) {
     pdl_begin();
-    __shared__ float s_sum[32][kJoinCols];
-    __shared__ int s_cnt[32][kJoinCols];
+    __shared__ __align__(16) float s_sum[32][kJoinCols];
+    __shared__ __align__(16) int s_cnt[32][kJoinCols];
     __shared__ int s_live[32];
     __shared__ double s_loss[kJoinCols / 32];
     __shared__ double cta_loss;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int e0 = blockIdx.x * kJoinCols;
+    const int at = min(e0 + 4 * lane, stride - 4);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     int c[4] = {0, 0, 0, 0};
-#pragma unroll 4
-    for (int i = warp; i < ctas; i += 32)
+    for (int i = warp; i < ctas; i += 32 * kJoinAhead) {
+        float4 f[kJoinAhead];
+        int4 n[kJoinAhead];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = e0 + 32 * k + lane;
-            const long long at = (long long)i * E + min(e, E - 1);
-            s[k] += part_sums[at];
-            c[k] += part_counts[at];
+        for (int j = 0; j < kJoinAhead; ++j) {
+            const long long row = (long long)min(i + 32 * j, ctas - 1) * stride + at;
+            f[j] = *reinterpret_cast<const float4*>(part_sums + row);
+            n[j] = *reinterpret_cast<const int4*>(part_counts + row);
         }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        s_sum[warp][32 * k + lane] = s[k];
-        s_cnt[warp][32 * k + lane] = c[k];
+        for (int j = 0; j < kJoinAhead; ++j) {
+            if (i + 32 * j >= ctas) break;
+            s[0] += f[j].x, s[1] += f[j].y, s[2] += f[j].z, s[3] += f[j].w;
+            c[0] += n[j].x, c[1] += n[j].y, c[2] += n[j].z, c[3] += n[j].w;
+        }
     }
+    *reinterpret_cast<float4*>(&s_sum[warp][4 * lane]) = make_float4(s[0], s[1], s[2], s[3]);
+    *reinterpret_cast<int4*>(&s_cnt[warp][4 * lane]) = make_int4(c[0], c[1], c[2], c[3]);
     int v = 0;
     for (int i = tid; i < ctas; i += kJoinThreads) v += part_live[i];
     v = __reduce_add_sync(0xffffffffu, v);
@@ -242,18 +251,22 @@ __global__ void __launch_bounds__(kJoinThreads)
         cta_loss = 0.0;
         for (int i = 0; i < kJoinCols / 32; ++i) cta_loss += s_loss[i];
     }
-    cluster.sync();
-    if (blockIdx.x == 0 && tid == 0) {
+    const int ranks = (int)cluster.num_blocks();
+    if (ranks > 1)
+        cluster.sync();
+    else
+        __syncthreads();
+    if (blockIdx.x == 0 && warp == 0) {
+        const int live = __reduce_add_sync(0xffffffffu, s_live[lane]);
         double total = 0.0;
-        int live = 0;
-        for (int k = 0; k < (int)cluster.num_blocks(); ++k)
-            total += *cluster.map_shared_rank(&cta_loss, k);
-        for (int w = 0; w < 32; ++w) live += s_live[w];
+        for (int k = 0; k < ranks; ++k) total += *cluster.map_shared_rank(&cta_loss, k);
         const double n = live;
-        *n_tokens = live;
-        *loss = live ? (float)((double)coef * E / (topk * n * n) * total) : 0.0f;
+        if (lane == 0) {
+            *n_tokens = live;
+            *loss = live ? (float)((double)coef * E * total / (topk * n * n)) : 0.0f;
+        }
     }
-    cluster.sync();                     // CTA 0 may still read the others' sums
+    if (ranks > 1) cluster.sync();      // CTA 0 may still read the others' sums
 }
 
 struct BalanceBwdArgs {
@@ -272,7 +285,6 @@ struct BalanceBwdArgs {
 template <typename LT, int LPT, int NV, bool VEC>
 __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const BalanceBwdArgs a) {
     pdl_begin();
-    __shared__ float s_factor;
     constexpr int kSubs = kBalThreads / LPT;
     const int sub = threadIdx.x / LPT, col = threadIdx.x % LPT;
     const LT* logits = static_cast<const LT*>(a.logits);
@@ -284,30 +296,24 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const Bala
     // Since sum_e p_e = 1, c may be taken relative to any constant; relative
     // to its mean (to an integer) the difference below loses no digits to the
     // part that all counts share.
+    float c[NV][4];
     int ci[NV][4];
-    long long total = 0;
+    float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int e = 4 * (LPT * i + col) + k;
-            ci[i][k] = e < a.E ? a.counts[e] : 0;
-            total += ci[i][k];
+            ci[i][k] = a.counts[min(e, a.E - 1)];
+            total += e < a.E ? (float)ci[i][k] : 0.0f;
         }
-#pragma unroll
-    for (int o = LPT / 2; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    const int mean = (int)(total / a.E);
-    float c[NV][4];
+    const int mean = (int)(lanes_sum<LPT>(total) / (float)a.E);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) c[i][k] = (float)(ci[i][k] - mean);
-    if (threadIdx.x == 0) {
-        const double n = *a.n_tokens;
-        s_factor = n > 0 ? (float)((double)*a.grad_loss * a.coef * a.E / (a.topk * n * n)) : 0.0f;
-    }
-    __syncthreads();
-    const float factor = s_factor;
+    const float n = (float)*a.n_tokens;
+    const float factor = n > 0.0f ? *a.grad_loss * a.coef * (float)a.E / (float)a.topk / n / n : 0.0f;
 
     const long long rounds = (a.T - (long long)blockIdx.x * kSubs + step - 1) / step;
     for (long long i0 = 0; i0 < rounds; ++i0) {
@@ -349,11 +355,14 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const Bala
 // Tokens that a CTA works on at once.
 int balance_tokens(int E) { return kBalThreads / (E <= 32 ? 8 : E <= 64 ? 16 : 32); }
 
-// Two rounds of tokens per CTA before a further CTA pays, four CTAs per SM at most.
+// Four rounds of tokens per CTA before a further CTA pays (the second launch reads a
+// row for every CTA), four CTAs per SM at most.
 int balance_ctas(int T, int E, int sms) {
-    const int per = 2 * balance_tokens(E);
+    const int per = 4 * balance_tokens(E);
     return std::max(1, std::min((int)(((long long)T + per - 1) / per), sms * 4));
 }
+
+int balance_stride(int E) { return (E + 3) / 4 * 4; }
 
 // Vector accesses: rows of whole vectors, each on a vector's boundary.
 bool balance_vec(const void* logits, long long ld, int E, int size, const void* out) {
@@ -385,7 +394,7 @@ using namespace ferret;
 
 extern "C" size_t ferret_moe_balance_loss_workspace_size(int T, int E) {
     if (T <= 0 || E <= 0 || E > kBalMaxE) return 0;
-    return (size_t)balance_ctas(T, E, kBalMaxCtas / 4) * (2 * (size_t)E + 1) * 4;
+    return (size_t)balance_ctas(T, E, kBalMaxCtas / 4) * (2 * (size_t)balance_stride(E) + 1) * 4;
 }
 
 extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dtype,
@@ -401,7 +410,7 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
         return FERRET_ERR_NULL;
     if (!aligned_to(logits, size) || !aligned_to(topk_ids, 4) || !aligned_to(loss, 4) ||
         !aligned_to(counts, 4) || !aligned_to(prob_sums, 4) || !aligned_to(n_tokens, 4) ||
-        !aligned_to(workspace, 4))
+        !aligned16(workspace))
         return FERRET_ERR_ALIGN;
     if (T > 0 && (!workspace || ws_bytes < ferret_moe_balance_loss_workspace_size(T, E)))
         return FERRET_ERR_WORKSPACE;
@@ -411,11 +420,12 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
     const cudaStream_t s = as_stream(stream);
     const int ctas = T ? balance_ctas(T, E, std::min(info->num_sms, kBalMaxCtas / 4)) : 0;
     float* sums = static_cast<float*>(workspace);
-    int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * E);
-    int32_t* live = cnts + (size_t)ctas * E;
+    const int stride = balance_stride(E);
+    int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * stride);
+    int32_t* live = cnts + (size_t)ctas * stride;
     if (T) {
         const BalanceArgs a{logits, ld, topk_ids, token_mask, T, E, topk,
-                            (flags & FERRET_ROUTE_SIGMOID) != 0, sums, cnts, live};
+                            (flags & FERRET_ROUTE_SIGMOID) != 0, sums, cnts, live, stride};
         rc = dtype == FERRET_BF16   ? run_balance<__nv_bfloat16>(a, ctas, s)
              : dtype == FERRET_FP16 ? run_balance<__half>(a, ctas, s)
                                     : run_balance<float>(a, ctas, s);
@@ -423,8 +433,8 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
     }
     const int join = (E + kJoinCols - 1) / kJoinCols;        // at most 8: one cluster
     return launch_kernel_cluster(moe_balance_join_kernel, dim3(join), dim3(kJoinThreads), 0, join,
-                                 s, sums, cnts, live, ctas, E, topk, coef, loss, counts, prob_sums,
-                                 n_tokens);
+                                 s, sums, cnts, live, ctas, stride, E, topk, coef, loss, counts,
+                                 prob_sums, n_tokens);
 }
 
 extern "C" int ferret_moe_balance_loss_backward(const float* grad_loss, const void* logits,

@@ -49,83 +49,93 @@ struct NormArgs {
     int tpr;   // threads per row: 16, 32 or a multiple of 32 (then one row per CTA)
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* p, int n, float v[8]) {
-    if (VEC) {
+// How a row's chunks of 8 columns are reached.
+enum Rows {
+    kElements,   // one by one
+    kVectors,    // every row of every tensor starts on a 16-byte boundary
+    kShifted,    // the rows of x, residual, y and residual_out share their distance from
+                 // one: chunks start there, `shift` columns before the row, and only
+                 // the row's two ends move one by one (and the weight, which stays in L1)
+};
+
+// Columns [at + lo, at + hi) of a chunk; hi <= lo: none.
+struct Piece {
+    int at, lo, hi;
+    __device__ __forceinline__ Piece(int c, int shift, int K) {
+        at = 8 * c - shift;
+        lo = max(0, -at);
+        hi = min(8, K - at);
+    }
+};
+
+template <typename T, int ROWS>
+__device__ __forceinline__ void load8(const T* row, const Piece& p, float v[8]) {
+    if (ROWS != kElements && (ROWS == kVectors || p.hi - p.lo == 8)) {
         Raw8<T> r;
 #pragma unroll
         for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-            r.w[i] = ld16_stream(reinterpret_cast<const uint4*>(p) + i);
+            r.w[i] = ld16_stream(reinterpret_cast<const uint4*>(row + p.at) + i);
         unpack8<T>(r, v);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = i >= p.lo && i < p.hi ? to_f32(row[p.at + i]) : 0.0f;
     }
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, int n, const float v[8]) {
-    if (VEC) {
+template <typename T, int ROWS>
+__device__ __forceinline__ void store8(T* row, const Piece& p, const float v[8]) {
+    if (ROWS != kElements && (ROWS == kVectors || p.hi - p.lo == 8)) {
         const Raw8<T> r = pack8<T>(v);
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
+            reinterpret_cast<uint4*>(row + p.at)[i] = r.w[i];
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = from_f32<T>(v[i]);
+            if (i >= p.lo && i < p.hi) row[p.at + i] = from_f32<T>(v[i]);
     }
 }
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_weight8(const NormArgs& a, int c, int n, float w[8]) {
-    if (a.weight_f32 && sizeof(T) != 4) {
-        const float* p = static_cast<const float*>(a.weight) + c * 8;
-        if (VEC) {
-            const float4 lo = __ldg(reinterpret_cast<const float4*>(p));
-            const float4 hi = __ldg(reinterpret_cast<const float4*>(p) + 1);
-            w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w;
-            w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = i < n ? p[i] : 0.0f;
-        }
-        return;
-    }
-    const T* p = static_cast<const T*>(a.weight) + c * 8;
+template <typename W, bool VEC>
+__device__ __forceinline__ void load_weight8(const W* w, const Piece& p, float v[8]) {
     if (VEC) {
-        Raw8<T> r;
+        Raw8<W> r;
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i)
-            r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        unpack8<T>(r, w);
+        for (int i = 0; i < (int)(sizeof(W) / 2); ++i)
+            r.w[i] = __ldg(reinterpret_cast<const uint4*>(w + p.at) + i);
+        unpack8<W>(r, v);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = i < n ? to_f32(p[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) v[i] = i >= p.lo && i < p.hi ? to_f32(w[p.at + i]) : 0.0f;
     }
 }
 
 // The outputs of a row from its s (v) and the sum of its squares (ss).  All lanes
 // of the warp take part; those without a live row or column store nothing.
-template <typename T, int NV, bool VEC>
-__device__ __forceinline__ void finish_row(const NormArgs& a, long long row, int tid, bool live,
-                                           const float (&v)[NV][8], float ss) {
+template <typename T, int NV, int ROWS>
+__device__ __forceinline__ void finish_row(const NormArgs& a, long long row, int tid, int shift,
+                                           bool live, const float (&v)[NV][8], float ss) {
     const int tpr = a.tpr, K = a.K;
     const float inv = 1.0f / sqrtf(ss / (float)K + a.eps);
-
     const int nk = K >> 7;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = i * tpr + tid, n = live ? K - c * 8 : 0;
+        const int c = i * tpr + tid;
+        const Piece p(c, shift, K);
+        const bool some = live && p.hi > p.lo;
         float y[8];
         float amax = 0.0f;
-        if (n > 0) {
+        if (some) {
             if (a.residual_out)
-                store8<T, VEC>(static_cast<T*>(a.residual_out) + row * K + c * 8, n, v[i]);
+                store8<T, ROWS>(static_cast<T*>(a.residual_out) + row * K, p, v[i]);
             float w[8];
-            load_weight8<T, VEC>(a, c, n, w);
+            if (sizeof(T) != 4 && a.weight_f32)
+                load_weight8<float, ROWS == kVectors>(static_cast<const float*>(a.weight), p, w);
+            else
+                load_weight8<T, ROWS == kVectors>(static_cast<const T*>(a.weight), p, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inv * w[j];
-            if (a.y) store8<T, VEC>(static_cast<T*>(a.y) + row * K + c * 8, n, y);
+            if (a.y) store8<T, ROWS>(static_cast<T*>(a.y) + row * K, p, y);
 #pragma unroll
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(y[j]));
         }
@@ -133,16 +143,14 @@ __device__ __forceinline__ void finish_row(const NormArgs& a, long long row, int
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1)          // within the 16 lanes of a 128-column block
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if (n <= 0) continue;
+        if (!some) continue;
         const Fp8Scale f = fp8_block_scale(amax, a.ue8m0);
         *reinterpret_cast<uint2*>(a.q + row * K + c * 8) = fp8_pack8(y, f.mul);
         if ((tid & 15) == 0) a.scale[row * nk + (c >> 4)] = f.scale;
     }
 }
 
-// VEC: K is a multiple of 8 and every row of x, residual, weight, y and
-// residual_out starts on a 16-byte boundary; otherwise elements move one by one.
-template <typename T, int NV, bool VEC>
+template <typename T, int NV, int ROWS>
 __global__ void __launch_bounds__(kNormMaxThreads) add_rms_norm_kernel(const NormArgs a) {
     pdl_begin();
     __shared__ float warp_sums[kNormMaxThreads / 32];
@@ -154,19 +162,21 @@ __global__ void __launch_bounds__(kNormMaxThreads) add_rms_norm_kernel(const Nor
     const bool live = row < a.T;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* res = static_cast<const T*>(a.residual) + row * a.ldr;
+    const int shift =
+        ROWS == kShifted ? (int)(reinterpret_cast<uintptr_t>(x) & 15u) / (int)sizeof(T) : 0;
 
     float v[NV][8];
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int c = i * tpr + tid, n = live ? K - c * 8 : 0;
+        const Piece p(i * tpr + tid, shift, K);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-        if (n <= 0) continue;
-        load8<T, VEC>(x + c * 8, n, v[i]);
+        if (!live || p.hi <= p.lo) continue;
+        load8<T, ROWS>(x, p, v[i]);
         if (a.residual) {
             float r[8];
-            load8<T, VEC>(res + c * 8, n, r);
+            load8<T, ROWS>(res, p, r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] += r[j];
         }
@@ -182,7 +192,7 @@ __global__ void __launch_bounds__(kNormMaxThreads) add_rms_norm_kernel(const Nor
         ss = (threadIdx.x & 31) < (tpr >> 5) ? warp_sums[threadIdx.x & 31] : 0.0f;
         ss = warp_sum(ss);
     }
-    finish_row<T, NV, VEC>(a, row, tid, live, v, ss);
+    finish_row<T, NV, ROWS>(a, row, tid, shift, live, v, ss);
 }
 
 // --------------------------------------------------------- the persistent form
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const NormArgs a
         }
         pos.advance(stages);
         ss = warp_sum(lane < (tpr >> 5) ? warp_sums[odd][lane] : 0.0f);
-        finish_row<T, NV, true>(a, row, tid, true, v, ss);
+        finish_row<T, NV, kVectors>(a, row, tid, 0, true, v, ss);
     }
     // a wait ran out: the copies in flight land before the CTA leaves (slots
     // that hold no further row end this wait by its time limit)
@@ -271,11 +281,14 @@ __global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const NormArgs a
 }
 
 template <typename T, int NV>
-int launch_norm(const NormArgs& a, bool vec, int threads, cudaStream_t s) {
+int launch_norm(const NormArgs& a, Rows rows, int threads, cudaStream_t s) {
     const int per_cta = a.tpr <= 32 ? threads / a.tpr : 1;
-    const dim3 grid((unsigned)(((long long)a.T + per_cta - 1) / per_cta));
-    return vec ? launch_kernel(add_rms_norm_kernel<T, NV, true>, grid, dim3(threads), 0, s, a)
-               : launch_kernel(add_rms_norm_kernel<T, NV, false>, grid, dim3(threads), 0, s, a);
+    const dim3 grid((unsigned)(((long long)a.T + per_cta - 1) / per_cta)), block(threads);
+    switch (rows) {
+        case kVectors: return launch_kernel(add_rms_norm_kernel<T, NV, kVectors>, grid, block, 0, s, a);
+        case kShifted: return launch_kernel(add_rms_norm_kernel<T, NV, kShifted>, grid, block, 0, s, a);
+        default: return launch_kernel(add_rms_norm_kernel<T, NV, kElements>, grid, block, 0, s, a);
+    }
 }
 
 template <typename T, int NV>
@@ -293,21 +306,27 @@ int launch_ring(const NormArgs& a, int ctas_per_sm, int stages, size_t smem, con
 }
 
 template <typename T>
-int run_norm(NormArgs& a, bool vec, const DeviceInfo* info, cudaStream_t s) {
-    const int chunks = (a.K + 7) / 8, sms = info->num_sms;
+int run_norm(NormArgs& a, Rows rows, const DeviceInfo* info, cudaStream_t s) {
+    // a shifted row may start late in its first chunk
+    int chunks = (a.K + 7 + (rows == kShifted ? 16 / (int)sizeof(T) - 1 : 0)) / 8;
+    if (chunks > kNormMaxNV * kNormMaxThreads) {
+        rows = kElements;
+        chunks = (a.K + 7) / 8;
+    }
+    const int sms = info->num_sms;
     if (chunks <= 32 * kNormMaxNV && a.T > sms * 8) {
         // short rows, many of them: a warp (or half of one) per row, 8 warps per CTA
         const int nv = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
         a.tpr = chunks <= 16 ? 16 : 32;
-        return nv == 1   ? launch_norm<T, 1>(a, vec, 256, s)
-               : nv == 2 ? launch_norm<T, 2>(a, vec, 256, s)
-                         : launch_norm<T, 4>(a, vec, 256, s);
+        return nv == 1   ? launch_norm<T, 1>(a, rows, 256, s)
+               : nv == 2 ? launch_norm<T, 2>(a, rows, 256, s)
+                         : launch_norm<T, 4>(a, rows, 256, s);
     }
     // Many long rows: the ring, with at least three rows in it.  An SM has 1 KB of
     // shared memory more than a CTA may use; a CTA takes 1 KB besides its own.
     const size_t stage = (size_t)a.K * sizeof(T) * (a.residual ? 2 : 1);
     const int room = info->max_smem_optin + 1024, own = 1024 + 512;
-    if (vec && a.T > sms * 8 && chunks <= 2 * 512 && 3 * stage + own <= (size_t)room) {
+    if (rows == kVectors && a.T > sms * 8 && chunks <= 2 * 512 && 3 * stage + own <= (size_t)room) {
         const int nv = chunks <= 256 ? 1 : 2;
         a.tpr = ((chunks + nv - 1) / nv + 31) / 32 * 32;
         const int ctas = std::min(2048 / a.tpr / 2, (int)(room / (3 * stage + own)));
@@ -320,9 +339,9 @@ int run_norm(NormArgs& a, bool vec, const DeviceInfo* info, cudaStream_t s) {
     int nv = a.T <= sms * 2 ? 1 : 2;
     while ((chunks + nv - 1) / nv > kNormMaxThreads) nv *= 2;
     a.tpr = std::max(64, ((chunks + nv - 1) / nv + 31) / 32 * 32);
-    return nv == 1   ? launch_norm<T, 1>(a, vec, a.tpr, s)
-           : nv == 2 ? launch_norm<T, 2>(a, vec, a.tpr, s)
-                     : launch_norm<T, 4>(a, vec, a.tpr, s);
+    return nv == 1   ? launch_norm<T, 1>(a, rows, a.tpr, s)
+           : nv == 2 ? launch_norm<T, 2>(a, rows, a.tpr, s)
+                     : launch_norm<T, 4>(a, rows, a.tpr, s);
 }
 
 }  // namespace
@@ -349,17 +368,23 @@ extern "C" int ferret_add_rms_norm(const void* x, long long ldx, const void* res
     DeviceInfo* info = nullptr;
     int rc = current_device(&info);
     if (rc != FERRET_OK) return rc;
-    // 16-byte accesses need every row of every tensor on a 16-byte boundary
-    const bool vec = K % 8 == 0 && aligned16(x) && aligned16(residual) && aligned16(y) &&
-                     aligned16(residual_out) && aligned16(weight) && (ldx * size) % 16 == 0 &&
-                     (!residual || (ldr * size) % 16 == 0);
+    auto off = [&](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; };
+    const bool together = (!residual || off(residual) == off(x)) && (!y || off(y) == off(x)) &&
+                          (!residual_out || off(residual_out) == off(x));
+    const size_t step = (size_t)K * size % 16;          // of the outputs' rows
+    const bool same_step = (T == 1 || (size_t)ldx * size % 16 == step) &&
+                           (!residual || T == 1 || (size_t)ldr * size % 16 == step);
+    const Rows rows = together && same_step && off(x) == 0 && off(weight) == 0 && K % 8 == 0
+                          ? kVectors
+                      : together && same_step && !q_fp8 ? kShifted
+                                                        : kElements;
     NormArgs a{x, ldx, residual, ldr, weight, weight_dtype == FERRET_FP32, T, K, eps, y,
                residual_out, static_cast<uint8_t*>(q_fp8), q_scale,
                (flags & FERRET_UE8M0_SCALES) != 0, 0};
     const cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case FERRET_BF16: return run_norm<__nv_bfloat16>(a, vec, info, s);
-        case FERRET_FP16: return run_norm<__half>(a, vec, info, s);
-        default: return run_norm<float>(a, vec, info, s);
+        case FERRET_BF16: return run_norm<__nv_bfloat16>(a, rows, info, s);
+        case FERRET_FP16: return run_norm<__half>(a, rows, info, s);
+        default: return run_norm<float>(a, rows, info, s);
     }
 }

@@ -408,7 +408,7 @@ FERRET_API int ferret_moe_route_backward(const float* grad_weights, const void* 
  * logits of -inf or NaN have p = 0.  logits `dtype` [T, E] with row stride ld,
  * topk_ids int32 [T, topk]; loss, n_tokens one element each.
  * The sums have a fixed order: same inputs on the same device, same bits.
- * workspace: ferret_moe_balance_loss_workspace_size(T, E) bytes, 4-byte
+ * workspace: ferret_moe_balance_loss_workspace_size(T, E) bytes, 16-byte
  * aligned, not shared by calls that can run at the same time.
  * Limits: E <= 1024.
  */

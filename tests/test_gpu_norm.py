@@ -119,6 +119,25 @@ def test_strided_and_unaligned_rows(ops, T):
     check(ops.add_rms_norm(x, w, None, quant=True), x, w, None, quant=True)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,K", [(1, 32768), (3, 32761), (1, 5), (1300, 33), (1300, 1021), (40, 4099)])
+@pytest.mark.parametrize("start", [0, 1, 3, 7])
+def test_rows_that_share_their_distance_from_a_boundary(ops, dtype, T, K, start):
+    """Odd row lengths and odd base addresses: every row starts somewhere else, the
+    same in x, residual and (when given) residual_out."""
+    def at(seed):
+        flat = make(1, T * K + 8, dtype, seed)[0].flatten()
+        return flat[start:start + T * K].view(T, K)
+
+    x, r, w = at(1), at(2), make(1, K, dtype, 3)[1]
+    check(ops.add_rms_norm(x, w, r), x, w, r)
+    out = at(4)
+    before = out.clone()
+    check(ops.add_rms_norm(x, w, r, residual_out=out), x, w, r)
+    check(ops.add_rms_norm(x, w), x, w, None)
+    assert not torch.equal(before, out)
+
+
 @pytest.mark.parametrize("T,K", [(3, 640), (1400, 2048), (1400, 513)])
 def test_residual_in_place(ops, T, K):
     x, w, r = make(T, K, torch.bfloat16, 8)

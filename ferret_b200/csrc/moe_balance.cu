@@ -19,23 +19,20 @@
 // each, and the next token's row is loaded before the current one is used.  The
 // forward kernel sums probabilities for its columns in registers over all its
 // tokens, so the only reduction across CTAs is one [CTAs, E] table of partial
-// sums and counts in the workspace.  A second launch (128 columns per CTA, one
-// cluster) adds its rows in a fixed order: no floating-point atomics, the same
-// bits every time.
+// sums and counts in the workspace.  A second launch (32 columns per CTA) adds its
+// rows in a fixed order, and the CTA that finishes last adds the CTAs' shares of the
+// loss: no floating-point atomics, the same bits every time.
 #include <algorithm>
-#include <cooperative_groups.h>
 
 #include "row_io.cuh"
 
 namespace ferret {
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr int kBalWarps = 8;
 constexpr int kBalThreads = kBalWarps * 32;
 constexpr int kBalMaxE = 1024;
-constexpr int kBalMaxCtas = 256 * 4;   // partial rows, on the largest device
+constexpr int kBalMaxCtas = 256 * 4;   // partial rows, on the largest device (the join reads 1024)
 
 struct BalanceArgs {
     const void* logits;
@@ -44,10 +41,10 @@ struct BalanceArgs {
     const uint8_t* mask;
     int T, E, topk;
     bool sigmoid;
-    float* part_sums;     // [ctas, stride]: stride is E, rounded up to whole vectors
-    int32_t* part_counts; // [ctas, stride]
+    float* part_sums;     // [ctas, E]
+    int32_t* part_counts; // [ctas, E]
     int32_t* part_live;   // [ctas]
-    int stride;
+    int32_t* done;        // CTAs of the second launch that are through: zeroed here
 };
 
 // A row's pieces as loaded: vector i of a lane holds columns 4 (LPT i + lane) ..+3.
@@ -85,7 +82,9 @@ __device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool s
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float z = p[i][k], e = expf(-fabsf(z)), inv = 1.0f / (1.0f + e);
+                const float z = p[i][k], e = expf(-fabsf(z));
+                float inv;                                // 1 ulp
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + e));
                 rest[i][k] = z >= 0.0f ? e * inv : inv;
                 p[i][k] = z >= 0.0f ? inv : e * inv;      // -inf: e = 0
                 sum += p[i][k];
@@ -175,98 +174,98 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceA
         float s = 0.0f;
 #pragma unroll
         for (int w = 0; w < kBalWarps; ++w) s += sums[w][e];
-        a.part_sums[(long long)blockIdx.x * a.stride + e] = s;
-        a.part_counts[(long long)blockIdx.x * a.stride + e] = counts[e];
+        a.part_sums[(long long)blockIdx.x * a.E + e] = s;
+        a.part_counts[(long long)blockIdx.x * a.E + e] = counts[e];
     }
-    if (threadIdx.x == 0) a.part_live[blockIdx.x] = live;
+    if (threadIdx.x == 0) {
+        a.part_live[blockIdx.x] = live;
+        if (blockIdx.x == 0) *a.done = 0;
+    }
 }
 
-// Adds the partial tables' rows in a fixed order and forms the loss.  A CTA
-// takes 128 columns, 4 adjacent ones per lane; warp w adds rows w, w + 32, ..., four of
-// them in flight at a time.
+// Adds the partial tables' rows in a fixed order and forms the loss.  A CTA takes
+// 32 columns; warp w adds rows w, w + 32, ..., eight of them in flight at a time.
 constexpr int kJoinThreads = 1024;
-constexpr int kJoinCols = 128;
-constexpr int kJoinAhead = 4;
+constexpr int kJoinAhead = 8;
+constexpr int kJoinMaxCtas = kBalMaxE / 32;
 
-__global__ void __launch_bounds__(kJoinThreads)
-    moe_balance_join_kernel(const float* part_sums, const int32_t* part_counts,
-                            const int32_t* part_live, int ctas, int stride, int E, int topk,
-                            float coef, float* loss, int32_t* counts, float* prob_sums,
-                            int32_t* n_tokens) {
+struct JoinArgs {
+    const float* part_sums;
+    const int32_t* part_counts;
+    const int32_t* part_live;
+    int32_t* done;
+    double* part_loss;    // [CTAs of this launch]
+    int ctas, E, topk;
+    float coef;
+    float* loss;
+    int32_t* counts;
+    float* prob_sums;
+    int32_t* n_tokens;
+};
+
+__global__ void __launch_bounds__(kJoinThreads) moe_balance_join_kernel(const JoinArgs a) {
     pdl_begin();
-    __shared__ __align__(16) float s_sum[32][kJoinCols];
-    __shared__ __align__(16) int s_cnt[32][kJoinCols];
+    __shared__ float s_sum[32][33];
+    __shared__ int s_cnt[32][33];
     __shared__ int s_live[32];
-    __shared__ double s_loss[kJoinCols / 32];
-    __shared__ double cta_loss;
-    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ bool last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int e0 = blockIdx.x * kJoinCols;
-    const int at = min(e0 + 4 * lane, stride - 4);
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    int c[4] = {0, 0, 0, 0};
-    for (int i = warp; i < ctas; i += 32 * kJoinAhead) {
-        float4 f[kJoinAhead];
-        int4 n[kJoinAhead];
+    const int e = blockIdx.x * 32 + lane, col = min(e, a.E - 1);
+    float s = 0.0f;
+    int c = 0;
+    for (int i = warp; i < a.ctas; i += 32 * kJoinAhead) {
+        float f[kJoinAhead];
+        int n[kJoinAhead];
 #pragma unroll
         for (int j = 0; j < kJoinAhead; ++j) {
-            const long long row = (long long)min(i + 32 * j, ctas - 1) * stride + at;
-            f[j] = *reinterpret_cast<const float4*>(part_sums + row);
-            n[j] = *reinterpret_cast<const int4*>(part_counts + row);
+            const long long at = (long long)min(i + 32 * j, a.ctas - 1) * a.E + col;
+            f[j] = a.part_sums[at];
+            n[j] = a.part_counts[at];
         }
 #pragma unroll
         for (int j = 0; j < kJoinAhead; ++j) {
-            if (i + 32 * j >= ctas) break;
-            s[0] += f[j].x, s[1] += f[j].y, s[2] += f[j].z, s[3] += f[j].w;
-            c[0] += n[j].x, c[1] += n[j].y, c[2] += n[j].z, c[3] += n[j].w;
+            s += i + 32 * j < a.ctas ? f[j] : 0.0f;
+            c += i + 32 * j < a.ctas ? n[j] : 0;
         }
     }
-    *reinterpret_cast<float4*>(&s_sum[warp][4 * lane]) = make_float4(s[0], s[1], s[2], s[3]);
-    *reinterpret_cast<int4*>(&s_cnt[warp][4 * lane]) = make_int4(c[0], c[1], c[2], c[3]);
-    int v = 0;
-    for (int i = tid; i < ctas; i += kJoinThreads) v += part_live[i];
-    v = __reduce_add_sync(0xffffffffu, v);
-    if (lane == 0) s_live[warp] = v;
+    s_sum[warp][lane] = s;
+    s_cnt[warp][lane] = c;
+    int live = tid < a.ctas ? a.part_live[tid] : 0;       // at most 1024 rows
+    live = __reduce_add_sync(0xffffffffu, live);
+    if (lane == 0) s_live[warp] = live;
     __syncthreads();
+    if (warp > 0) return;
+    s = 0.0f;
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+        s += s_sum[w][lane];
+        c += s_cnt[w][lane];
+    }
     double part = 0.0;
-    if (tid < kJoinCols) {
-        float sum = 0.0f;
-        int cnt = 0;
-#pragma unroll
-        for (int w = 0; w < 32; ++w) {
-            sum += s_sum[w][tid];
-            cnt += s_cnt[w][tid];
-        }
-        if (e0 + tid < E) {
-            prob_sums[e0 + tid] = sum;
-            counts[e0 + tid] = cnt;
-            part = (double)cnt * (double)sum;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-        if (lane == 0) s_loss[warp] = part;
+    if (e < a.E) {
+        a.prob_sums[e] = s;
+        a.counts[e] = c;
+        part = (double)c * (double)s;
     }
-    __syncthreads();
-    if (tid == 0) {
-        cta_loss = 0.0;
-        for (int i = 0; i < kJoinCols / 32; ++i) cta_loss += s_loss[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
+    if (lane == 0) {
+        a.part_loss[blockIdx.x] = part;
+        __threadfence();
+        last = atomicAdd(a.done, 1) == (int)gridDim.x - 1;
+        __threadfence();
     }
-    const int ranks = (int)cluster.num_blocks();
-    if (ranks > 1)
-        cluster.sync();
-    else
-        __syncthreads();
-    if (blockIdx.x == 0 && warp == 0) {
-        const int live = __reduce_add_sync(0xffffffffu, s_live[lane]);
+    __syncwarp();
+    if (!last) return;
+    live = __reduce_add_sync(0xffffffffu, s_live[lane]);
+    if (lane == 0) {
         double total = 0.0;
-        for (int k = 0; k < ranks; ++k) total += *cluster.map_shared_rank(&cta_loss, k);
+        for (int k = 0; k < (int)gridDim.x; ++k) total += __ldcg(a.part_loss + k);
         const double n = live;
-        if (lane == 0) {
-            *n_tokens = live;
-            *loss = live ? (float)((double)coef * E * total / (topk * n * n)) : 0.0f;
-        }
+        *a.n_tokens = live;
+        *a.loss = live ? (float)((double)a.coef * a.E * total / (a.topk * n * n)) : 0.0f;
     }
-    if (ranks > 1) cluster.sync();      // CTA 0 may still read the others' sums
 }
 
 struct BalanceBwdArgs {
@@ -355,14 +354,12 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const Bala
 // Tokens that a CTA works on at once.
 int balance_tokens(int E) { return kBalThreads / (E <= 32 ? 8 : E <= 64 ? 16 : 32); }
 
-// Four rounds of tokens per CTA before a further CTA pays (the second launch reads a
+// Two rounds of tokens per CTA before a further CTA pays (the second launch reads a
 // row for every CTA), four CTAs per SM at most.
 int balance_ctas(int T, int E, int sms) {
-    const int per = 4 * balance_tokens(E);
+    const int per = 2 * balance_tokens(E);
     return std::max(1, std::min((int)(((long long)T + per - 1) / per), sms * 4));
 }
-
-int balance_stride(int E) { return (E + 3) / 4 * 4; }
 
 // Vector accesses: rows of whole vectors, each on a vector's boundary.
 bool balance_vec(const void* logits, long long ld, int E, int size, const void* out) {
@@ -394,7 +391,8 @@ using namespace ferret;
 
 extern "C" size_t ferret_moe_balance_loss_workspace_size(int T, int E) {
     if (T <= 0 || E <= 0 || E > kBalMaxE) return 0;
-    return (size_t)balance_ctas(T, E, kBalMaxCtas / 4) * (2 * (size_t)balance_stride(E) + 1) * 4;
+    return kJoinMaxCtas * sizeof(double) + 16 +
+           (size_t)balance_ctas(T, E, kBalMaxCtas / 4) * (2 * (size_t)E + 1) * 4;
 }
 
 extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dtype,
@@ -418,23 +416,32 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
     int rc = current_device(&info);
     if (rc != FERRET_OK) return rc;
     const cudaStream_t s = as_stream(stream);
-    const int ctas = T ? balance_ctas(T, E, std::min(info->num_sms, kBalMaxCtas / 4)) : 0;
-    float* sums = static_cast<float*>(workspace);
-    const int stride = balance_stride(E);
-    int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * stride);
-    int32_t* live = cnts + (size_t)ctas * stride;
-    if (T) {
-        const BalanceArgs a{logits, ld, topk_ids, token_mask, T, E, topk,
-                            (flags & FERRET_ROUTE_SIGMOID) != 0, sums, cnts, live, stride};
-        rc = dtype == FERRET_BF16   ? run_balance<__nv_bfloat16>(a, ctas, s)
-             : dtype == FERRET_FP16 ? run_balance<__half>(a, ctas, s)
-                                    : run_balance<float>(a, ctas, s);
-        if (rc != FERRET_OK) return rc;
+    if (T == 0) {
+        if (cudaMemsetAsync(loss, 0, 4, s) != cudaSuccess ||
+            cudaMemsetAsync(counts, 0, (size_t)E * 4, s) != cudaSuccess ||
+            cudaMemsetAsync(prob_sums, 0, (size_t)E * 4, s) != cudaSuccess ||
+            cudaMemsetAsync(n_tokens, 0, 4, s) != cudaSuccess) {
+            cudaGetLastError();
+            return FERRET_ERR_CUDA;
+        }
+        return FERRET_OK;
     }
-    const int join = (E + kJoinCols - 1) / kJoinCols;        // at most 8: one cluster
-    return launch_kernel_cluster(moe_balance_join_kernel, dim3(join), dim3(kJoinThreads), 0, join,
-                                 s, sums, cnts, live, ctas, stride, E, topk, coef, loss, counts,
-                                 prob_sums, n_tokens);
+    const int ctas = balance_ctas(T, E, std::min(info->num_sms, kBalMaxCtas / 4));
+    // loss shares, the counter, then the tables
+    double* shares = static_cast<double*>(workspace);
+    int32_t* done = reinterpret_cast<int32_t*>(shares + kJoinMaxCtas);
+    float* sums = reinterpret_cast<float*>(done + 4);
+    int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * E);
+    int32_t* live = cnts + (size_t)ctas * E;
+    const BalanceArgs a{logits, ld, topk_ids, token_mask, T, E, topk,
+                        (flags & FERRET_ROUTE_SIGMOID) != 0, sums, cnts, live, done};
+    rc = dtype == FERRET_BF16   ? run_balance<__nv_bfloat16>(a, ctas, s)
+         : dtype == FERRET_FP16 ? run_balance<__half>(a, ctas, s)
+                                : run_balance<float>(a, ctas, s);
+    if (rc != FERRET_OK) return rc;
+    const JoinArgs j{sums, cnts, live, done, shares, ctas, E, topk, coef, loss, counts, prob_sums,
+                     n_tokens};
+    return launch_kernel(moe_balance_join_kernel, dim3((E + 31) / 32), dim3(kJoinThreads), 0, s, j);
 }
 
 extern "C" int ferret_moe_balance_loss_backward(const float* grad_loss, const void* logits,

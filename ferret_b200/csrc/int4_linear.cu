@@ -31,7 +31,9 @@
 // tensor-map boxes (word rows and token rows of 128 bytes, 128-byte swizzle;
 // the groups' scale rows); the math groups take the stages in turn.  Bytes in
 // flight thus cost no registers, and few copies carry them: one bulk copy per
-// 512-byte word row left the copy unit at half the HBM rate.  The eight lanes of
+// 512-byte word row left the copy unit at half the HBM rate.  Two CTAs per SM: with
+// three, 72 registers a thread made the compiler compute fragments and scales again
+// (158 warp instructions per 32 x 32 block for 16 tokens against 130).  The eight lanes of
 // a 16-byte shared-memory read phase hold r = 2q, 2q + 1 and all c; with r
 // standing for 16-byte piece (token) q or q + 4, the swizzle spreads them over
 // all banks.
@@ -63,9 +65,8 @@ constexpr int kLinMaxCluster = 8;
 // belongs to the same group: a group that met a slot only every other lap could
 // take the completion of the lap before last for its own (the wait sees a lap's
 // parity, not its number).
-template <int NT>
-constexpr int kLinStages = NT == 2 ? 4 : 6;
-static_assert(kLinStages<1> % kLinKGroups == 0 && kLinStages<2> % kLinKGroups == 0);
+constexpr int kLinStages = 6;
+static_assert(kLinStages % kLinKGroups == 0);
 // Stage layout: a box of word rows per column warp, token rows in boxes of 64
 // activations, scale rows; boxes on 1024 bytes (the swizzle's period).
 constexpr int kLinWordBox = 4 * kLinDepth * 128;
@@ -98,6 +99,10 @@ struct Half2Ops<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
         return bf16x2_sub(a, b);
     }
+    static __device__ __forceinline__ void unpack(uint2 v, float (&f)[4]) {
+        f[0] = __uint_as_float(v.x << 16), f[1] = __uint_as_float(v.x & 0xFFFF0000u);
+        f[2] = __uint_as_float(v.y << 16), f[3] = __uint_as_float(v.y & 0xFFFF0000u);
+    }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1, const float (&c)[4]) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
@@ -115,6 +120,11 @@ struct Half2Ops<__half> {
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
         return d;
     }
+    static __device__ __forceinline__ void unpack(uint2 v, float (&f)[4]) {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x)),
+                     b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+        f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+    }
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                                uint32_t b1, const float (&c)[4]) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
@@ -130,7 +140,7 @@ __device__ __forceinline__ int spread(int r) { return (r >> 1) + 4 * (r & 1); }
 
 // NT: groups of 8 tokens that one pass over the weights serves.
 template <typename T, int NT, bool ZERO>
-__global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(kLinThreads, 2)
     int4_linear_kernel(const __grid_constant__ CUtensorMap w_map,
                        const __grid_constant__ CUtensorMap x_map,
                        const __grid_constant__ CUtensorMap s_map, const LinearArgs a,
@@ -140,7 +150,7 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~(uintptr_t)1023);
-    __shared__ uint64_t full[kLinStages<NT>], empty[kLinStages<NT>];
+    __shared__ uint64_t full[kLinStages], empty[kLinStages];
     __shared__ int abort_flag;
     cg::cluster_group cluster = cg::this_cluster();
     const int splits = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
@@ -149,7 +159,7 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
     const int t0 = blockIdx.z * (NT * 8);
     const int tokens = min(a.T - t0, NT * 8);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kLinStages<NT>; ++i) {
+        for (int i = 0; i < kLinStages; ++i) {
             mbar_init(smem_addr(&full[i]), 1);
             mbar_init(smem_addr(&empty[i]), kLinColWarps);
         }
@@ -181,8 +191,8 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
         const uint32_t bytes = kLinColWarps * kLinWordBox + kLinDepth / 2 * kLinTokenBox<NT> +
                                a.scale_rows * kLinScaleRow;
         RingPos pos;
-        for (int s = 0; s < stages; ++s, pos.advance(kLinStages<NT>)) {
-            if (s >= kLinStages<NT> &&
+        for (int s = 0; s < stages; ++s, pos.advance(kLinStages)) {
+            if (s >= kLinStages &&
                 !__all_sync(0xffffffffu, mbar_wait(smem_addr(&empty[pos.slot]), pos.phase ^ 1u,
                                                    &abort_flag, ctl, 23)))
                 break;
@@ -210,7 +220,7 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
         const int nc = min(n0 + 32 * cw + 4 * piece, a.N - 4);
         const int swz[2] = {(piece ^ c) << 4, (piece ^ (4 + c)) << 4};
         RingPos pos;
-        for (int s = 0; s < stages; ++s, pos.advance(kLinStages<NT>)) {
+        for (int s = 0; s < stages; ++s, pos.advance(kLinStages)) {
             if (s % kLinKGroups != kg) continue;
             // Blocks past K multiply zero-filled activations with zero-filled scales.
             const int b = (s0 + s) * kLinDepth;
@@ -234,8 +244,8 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
                 const int row = a.even_groups ? d * a.scale_rows >> 2
                                                                   : group_of(b + d) - group_of(b);
                 const uint2 sv = *reinterpret_cast<const uint2*>(ss + row * kLinScaleRow);
-                T e[4];
-                memcpy(e, &sv, 8);
+                float sf[4];
+                Ops::unpack(sv, sf);
                 const uint32_t word[4] = {wv.x, wv.y, wv.z, wv.w};
                 uint32_t q4[4][4];      // [column][nibble pair j, j + 4]
 #pragma unroll
@@ -270,7 +280,7 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
 #pragma unroll
                         for (int q = 0; q < 4; ++q)
                             sum[i][h][q] =
-                                fmaf(to_f32(e[2 * h + (q >> 1)]), acc[q], sum[i][h][q]);
+                                fmaf(sf[2 * h + (q >> 1)], acc[q], sum[i][h][q]);
                     }
                 }
             }
@@ -282,8 +292,8 @@ __global__ void __launch_bounds__(kLinThreads, NT <= 2 ? 3 : 2)
     // copies have to land before their memory is used again.
     __syncthreads();
     if (abort_flag && warp == kLinMath)
-        for (int s = max(0, issued - kLinStages<NT>); s < issued; ++s)
-            mbar_wait(smem_addr(&full[s % kLinStages<NT>]), (s / kLinStages<NT>) & 1, &abort_flag, ctl, 24,
+        for (int s = max(0, issued - kLinStages); s < issued; ++s)
+            mbar_wait(smem_addr(&full[s % kLinStages]), (s / kLinStages) & 1, &abort_flag, ctl, 24,
                       false);
     __syncthreads();
 
@@ -343,7 +353,7 @@ int launch_linear(const LinearIn& in, const LinearArgs& a, int splits, const Dev
                            a.scale_rows, false)) != FERRET_OK)
         return rc;
     const dim3 grid(splits, (a.N + kLinCols - 1) / kLinCols, (a.T + NT * 8 - 1) / (NT * 8));
-    constexpr size_t smem = kLinStages<NT> * kLinStageBytes<NT> + 1024;
+    constexpr size_t smem = kLinStages * kLinStageBytes<NT> + 1024;
     static_assert(smem >= kLinKGroups * NT * 8 * kLinCols * sizeof(float) + 1024);
     auto kern = int4_linear_kernel<T, NT, ZERO>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
@@ -364,11 +374,12 @@ int launch_linear(const LinearIn& in, const LinearArgs& a, int splits, const Dev
 
 template <typename T>
 int run_linear(const LinearIn& in, const LinearArgs& a, const DeviceInfo* info, cudaStream_t s) {
-    // The fewest splits that give every SM about three CTAs in turn, as long as a
-    // CTA keeps four stages of K.
+    // The fewest splits that give every SM a CTA, as long as a CTA keeps four
+    // stages of K: a split costs its two cluster barriers (16 tokens x 7168 x
+    // 32768: 53 us unsplit, 57 us split in two or four).
     const long long tiles = ((long long)a.N + kLinCols - 1) / kLinCols;
     int splits = 1;
-    while (splits < kLinMaxCluster && tiles * splits < (long long)info->num_sms * 3 &&
+    while (splits < kLinMaxCluster && tiles * splits < (long long)info->num_sms &&
            a.K / 32 >= splits * 2 * 4 * kLinDepth)
         splits *= 2;
     if (a.T <= 8) return launch_linear<T, 1>(in, a, splits, info, s);

@@ -62,6 +62,14 @@ __device__ __forceinline__ RowRaw<LT, NV> load_row(const LT* row, int E) {
     return r;
 }
 
+// e^v from its exponent in base 2: the ex2 approximation, relative error 2^-22.
+__device__ __forceinline__ float exp2_fast(float v) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v));
+    return e;
+}
+constexpr float kLog2E = 1.44269504f;
+
 // Its probabilities (all zero for a row of closed logits), and the factor that
 // the scoring adds to the gradient: 1 - sigmoid(z), or 1 for the softmax.
 template <typename LT, int LPT, int NV>
@@ -82,7 +90,7 @@ __device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool s
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float z = p[i][k], e = expf(-fabsf(z));
+                const float z = p[i][k], e = exp2_fast(-kLog2E * fabsf(z));
                 float inv;                                // 1 ulp
                 asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + e));
                 rest[i][k] = z >= 0.0f ? e * inv : inv;
@@ -96,7 +104,7 @@ __device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool s
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                p[i][k] = expf(p[i][k] - shift);
+                p[i][k] = exp2_fast((p[i][k] - shift) * kLog2E);
                 rest[i][k] = 1.0f;
                 sum += p[i][k];
             }

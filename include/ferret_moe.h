@@ -406,7 +406,10 @@ FERRET_API int ferret_moe_route_backward(const float* grad_weights, const void* 
  *               FERRET_ROUTE_SIGMOID, sigmoids divided by their sum over e
  *   n_tokens = V
  *   loss = coef * E / (topk * V^2) * sum_e counts[e] * prob_sums[e]  (0 if V == 0)
- * logits of -inf or NaN have p = 0.  logits `dtype` [T, E] with row stride ld,
+ * logits of -inf or NaN have p = 0, and so have with FERRET_ROUTE_SIGMOID the rows
+ * that hold nothing but these and `dtype`'s lowest finite value (a mask that leaves
+ * nothing); every other row of finite logits, however far from zero, has
+ * probabilities that add up to 1.  logits `dtype` [T, E] with row stride ld,
  * topk_ids int32 [T, topk]; loss, n_tokens one element each.
  * The sums have a fixed order: same inputs on the same device, same bits.
  * workspace: ferret_moe_balance_loss_workspace_size(T, E) bytes, 16-byte

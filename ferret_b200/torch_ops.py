@@ -35,11 +35,11 @@ and, for the operators around the expert layer (no reference counterpart):
 * ``ferret_moe::int4_linear(Tensor x, Tensor w, Tensor w_scale, Tensor?
   w_zero=None, Tensor? bias=None) -> Tensor``.
 
-A differentiable call is refused while its stream is being captured into a CUDA
-graph, forward and backward: a captured backward pass that meets gradient
-accumulators of an eager graph on another stream breaks the capture beyond
-repair.  Captured training steps call ``ops.moe_route``,
-``ops.moe_route_backward``, ``ops.moe_balance_loss`` and
+A second derivative through these two raises.  A differentiable call is refused
+while its stream is being captured into a CUDA graph, forward and backward: a
+captured backward pass that meets gradient accumulators of an eager graph on
+another stream breaks the capture beyond repair.  Captured training steps call
+``ops.moe_route``, ``ops.moe_route_backward``, ``ops.moe_balance_loss`` and
 ``ops.moe_balance_loss_backward``, which record no autograd graph.
 
 Every operator runs the CUDA library (CUDA tensors only); importing this
@@ -140,6 +140,22 @@ def _not_captured(name):
                            f"graph capture: capture ops.{name} and ops.{name}_backward instead")
 
 
+class _Once(torch.autograd.Function):
+    """A backward function's result, tied to what it was formed from.  With
+    create_graph=True a second derivative through it raises; as a plain tensor it
+    would count as a constant."""
+
+    @staticmethod
+    def forward(ctx, name, backward, *inputs):
+        ctx.name = name
+        return backward(*inputs)
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"torch.ops.ferret_moe.{ctx.name} can be differentiated once only: its "
+                           "backward pass has no gradient of its own")
+
+
 def _route_setup(ctx, inputs, output):
     _not_captured("moe_route")
     logits, _, scoring, _, _, _, _, renormalize, scale, _ = inputs
@@ -154,7 +170,8 @@ def _route_backward(ctx, grad_weights, _):
     logits, ids = ctx.saved_tensors
     grad = None
     if grad_weights is not None:
-        grad = ops.moe_route_backward(grad_weights.contiguous(), logits, ids, **ctx.form)
+        grad = _Once.apply("moe_route", lambda g, z: ops.moe_route_backward(
+            g.contiguous(), z, ids, **ctx.form), grad_weights, logits)
     return grad, *[None] * 9
 
 
@@ -173,8 +190,9 @@ def _balance_backward(ctx, grad_loss, *_):
     topk, coef, scoring = ctx.form
     grad = None
     if grad_loss is not None:
-        grad = ops.moe_balance_loss_backward(grad_loss.contiguous(), logits, counts, n_tokens, topk,
-                                             coef, scoring=scoring, token_mask=token_mask)
+        grad = _Once.apply("moe_balance_loss", lambda g, z: ops.moe_balance_loss_backward(
+            g.contiguous(), z, counts, n_tokens, topk, coef, scoring=scoring,
+            token_mask=token_mask), grad_loss, logits)
     return grad, None, None, None, None
 
 

@@ -120,7 +120,8 @@ def host():
             raise ImportError(
                 f"ferret_b200 host module not usable ({e}); build it with "
                 "`python -m ferret_b200.build`") from e
-        _host.set_check(check)
+        from . import ops
+        _host.set_callbacks(check, ops._no_backward)
         _HOST = _host
     return _HOST
 

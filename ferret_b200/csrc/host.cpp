@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -23,6 +24,7 @@
 namespace {
 
 PyObject* g_check = nullptr;      // _lib.check(rc, name): raises for rc != 0
+PyObject* g_no_backward = nullptr;   // ops._no_backward(name, outs, given, *inputs)
 
 [[noreturn]] void fail(PyObject* type, const char* format, ...) {
     va_list v;
@@ -147,6 +149,37 @@ void expect(Py_ssize_t n, Py_ssize_t want) {
     if (n != want) fail(PyExc_TypeError, "expected %zd arguments, got %zd", want, n);
 }
 
+// `outs` (stolen) of an operator without a backward pass, as it is returned: where
+// autograd records and a tensor of `inputs` requires a gradient, tied to them, so that
+// a gradient raises and is not lost.  given: the output that the caller passed in.
+PyObject* no_backward(const char* name, PyObject* outs, PyObject* given,
+                      std::initializer_list<PyObject*> inputs) {
+    bool any = false;
+    if (at::GradMode::is_enabled())
+        for (PyObject* o : inputs) any = any || (!none(o) && THPVariable_Unpack(o).requires_grad());
+    if (!any) return outs;
+    PyObject* args = PyTuple_New((Py_ssize_t)(3 + inputs.size()));
+    PyObject* label = args ? PyUnicode_FromString(name) : nullptr;
+    if (!label) {
+        Py_XDECREF(args);
+        Py_DECREF(outs);
+        throw python_error();
+    }
+    PyTuple_SET_ITEM(args, 0, label);
+    PyTuple_SET_ITEM(args, 1, outs);
+    Py_INCREF(given);
+    PyTuple_SET_ITEM(args, 2, given);
+    Py_ssize_t i = 3;
+    for (PyObject* o : inputs) {
+        Py_INCREF(o);
+        PyTuple_SET_ITEM(args, i++, o);
+    }
+    PyObject* r = PyObject_CallObject(g_no_backward, args);
+    Py_DECREF(args);
+    if (!r) throw python_error();
+    return r;
+}
+
 int scoring_flags(PyObject* scoring, bool renorm) {
     int flags = renorm ? FERRET_ROUTE_RENORM : 0;
     if (PyUnicode_Check(scoring)) {
@@ -197,7 +230,8 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               quant ? s.data_ptr<float>() : nullptr,
                               truth(a[5]) ? FERRET_UE8M0_SCALES : 0, on.stream),
           "ferret_add_rms_norm");
-    return tuple({y, residual_out, q, s});
+    return no_backward("ops.add_rms_norm", tuple({y, residual_out, q, s}), a[7],
+                       {a[0], a[1], a[2], a[7]});
     END_HANDLE_TH_ERRORS
 }
 
@@ -330,14 +364,19 @@ PyObject* int4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check(ferret_int4_linear(x.data_ptr(), ldx, (const int32_t*)wp, sp, (const int32_t*)zp, bp, dt,
                              (int)T, (int)K, (int)N, (int)(K / groups), op, on.stream),
           "ferret_int4_linear");
-    return wrap(out);
+    return no_backward("ops.int4_linear", wrap(out), a[5], {a[0], a[2], a[4], a[5]});
     END_HANDLE_TH_ERRORS
 }
 
-PyObject* set_check(PyObject*, PyObject* f) {
-    Py_INCREF(f);
-    Py_XSETREF(g_check, f);
+PyObject* set_callbacks(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    expect(n, 2);
+    Py_INCREF(a[0]);
+    Py_XSETREF(g_check, a[0]);
+    Py_INCREF(a[1]);
+    Py_XSETREF(g_no_backward, a[1]);
     Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
 }
 
 #define FERRET_FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
@@ -347,7 +386,7 @@ PyMethodDef methods[] = {FERRET_FN(add_rms_norm),
                          FERRET_FN(moe_balance_loss),
                          FERRET_FN(moe_balance_loss_backward),
                          FERRET_FN(int4_linear),
-                         {"set_check", set_check, METH_O, nullptr},
+                         FERRET_FN(set_callbacks),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ferret_b200._host",

@@ -404,8 +404,39 @@ def moe_wna16_w13(hidden: torch.Tensor, weights: Int4W13Weights, topk_ids: torch
 
 # Around the expert layer: the functions below hand their arguments to the extension
 # module, which checks them, allocates the outputs and makes the C-ABI call on
-# the tensors' device and that device's current stream.  They record no autograd
-# graph; torch_ops registers the differentiable forms.
+# the tensors' device and that device's current stream.  moe_route and
+# moe_balance_loss record no autograd graph (they have backward functions beside them,
+# and differentiable forms in torch_ops).  The others have no backward pass: where
+# autograd is recording and an input requires a gradient, their results carry
+# a graph node that raises when a gradient reaches it.
+
+class _NoBackward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, name, given, outs, *inputs):
+        ctx.name = name
+        if given is not None:
+            ctx.mark_dirty(given)
+        return outs
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError(f"{ctx.name} has no backward pass: call it under torch.no_grad(), or on "
+                           "detached tensors, where no gradient has to go through it")
+
+
+def _no_backward(name, outs, given, *inputs):
+    """outs (a tensor, or a tuple that may hold None), tied to the inputs; `given`: the
+    one of them that the caller passed in to be written."""
+    inputs = [t for t in inputs if t is not None]
+    if given is None:
+        return _NoBackward.apply(name, None, outs, *inputs)
+    tied = _NoBackward.apply(name, given, given, *inputs)      # one output: it may be a view
+    if outs is given:
+        return tied
+    rest = tuple(None if t is given else t for t in outs)
+    rest = _NoBackward.apply(name, None, rest, *inputs)
+    return tuple(tied if t is given else r for t, r in zip(outs, rest))
+
 
 # --------------------------------------------------------- norm with FP8 rows
 
@@ -420,7 +451,8 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     residual_out, q, scale): y None with ``normed=False``, residual_out (the
     rounded s) None without a residual, q and scale None without ``quant``.
     Pass ``residual_out`` to have it written there; it may be ``residual`` or
-    ``x`` itself.  With ``quant`` K must be a multiple of 128; K <= 32768."""
+    ``x`` itself.  With ``quant`` K must be a multiple of 128; K <= 32768.  No
+    backward pass."""
     return host().add_rms_norm(x, weight, residual, eps, quant, use_ue8m0, normed, residual_out)
 
 
@@ -492,7 +524,7 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     g is a multiple of 32, N of 8; x's rows may be strided (by a multiple of 8
     elements).  Scales are applied in fp32 to the groups' fp32 sums.  Every 32
     tokens read the weights once: the decode form; large batches go through
-    ``moe_wna16_w13`` or a dequantized GEMM."""
+    ``moe_wna16_w13`` or a dequantized GEMM.  No backward pass."""
     return host().int4_linear(x, w, w_scale, w_zero, bias, out)
 
 
@@ -530,7 +562,8 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
     x, residual bf16 [T, H]; ``routing`` holds ``moe_route``'s keyword
     arguments.  Returns (out bf16 [T, H], residual_out, ids, logits): out is the
     layer's contribution, still to be added to residual_out (x itself without a
-    residual), and logits with ids are what ``moe_balance_loss`` takes."""
+    residual), and logits with ids are what ``moe_balance_loss`` takes.  No backward
+    pass."""
     _need(x, torch.bfloat16, "x", 2)
     _need(gate_weight, torch.bfloat16, "gate_weight", 2)
     T, H = x.shape
@@ -546,6 +579,14 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
                     ("W2", W2), ("W2_scale", W2_scale)):
         if t.device != x.device:
             raise ValueError(f"{name} must be on the device of x")
+    tied = (x, residual, norm_weight, gate_weight)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tied):
+        with torch.no_grad():
+            out, res, ids, logits = fp8_moe_block(x, residual, norm_weight, gate_weight, W13,
+                                                  W13_scale, W2, W2_scale, topk, eps=eps, **routing)
+        made = _no_backward("ops.fp8_moe_block", (out, None if residual is None else res, logits),
+                            None, *tied)
+        return made[0], x if residual is None else made[1], ids, made[2]
     with torch.cuda.device(x.device):
         y, res, q, s = add_rms_norm(x, norm_weight, residual, eps, quant=True)
         logits = torch.mm(y, gate_weight.t(), out_dtype=torch.float32)

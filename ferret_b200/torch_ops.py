@@ -35,11 +35,14 @@ and, for the operators around the expert layer (no reference counterpart):
 * ``ferret_moe::int4_linear(Tensor x, Tensor w, Tensor w_scale, Tensor?
   w_zero=None, Tensor? bias=None) -> Tensor``.
 
-A second derivative through these two raises.  A differentiable call is refused
-while its stream is being captured into a CUDA graph, forward and backward: a
-captured backward pass that meets gradient accumulators of an eager graph on
-another stream breaks the capture beyond repair.  Captured training steps call
-``ops.moe_route``, ``ops.moe_route_backward``, ``ops.moe_balance_loss`` and
+The norms and ``int4_linear`` have no backward pass: a gradient that reaches
+their results raises.
+A second derivative through the router or the balance loss raises.  A
+differentiable call of theirs is refused while its stream is being captured into
+a CUDA graph, forward and backward: a captured backward pass that meets gradient
+accumulators of an eager graph on another stream breaks the capture beyond
+repair.  Captured training steps call ``ops.moe_route``,
+``ops.moe_route_backward``, ``ops.moe_balance_loss`` and
 ``ops.moe_balance_loss_backward``, which record no autograd graph.
 
 Every operator runs the CUDA library (CUDA tensors only); importing this
@@ -196,6 +199,14 @@ def _balance_backward(ctx, grad_loss, *_):
     return grad, None, None, None, None
 
 
+def _no_backward(name):
+    def backward(ctx, *_):
+        raise RuntimeError(f"torch.ops.ferret_moe.{name} has no backward pass: call it under "
+                           "torch.no_grad(), or on detached tensors, where no gradient has to go "
+                           "through it")
+    return backward
+
+
 _LIB.impl("add_rms_norm", _norm, "CUDA")
 _LIB.impl("add_rms_norm_fp8", _norm_fp8, "CUDA")
 _LIB.impl("moe_route", _route, "CUDA")
@@ -205,3 +216,5 @@ torch.library.register_autograd("ferret_moe::moe_route", _route_backward,
                                 setup_context=_route_setup, lib=_LIB)
 torch.library.register_autograd("ferret_moe::moe_balance_loss", _balance_backward,
                                 setup_context=_balance_setup, lib=_LIB)
+for _name in ("add_rms_norm", "add_rms_norm_fp8", "int4_linear"):
+    torch.library.register_autograd(f"ferret_moe::{_name}", _no_backward(_name), lib=_LIB)

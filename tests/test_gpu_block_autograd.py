@@ -44,3 +44,104 @@ def test_second_derivatives_raise(F, op, outer):
             torch.autograd.grad(grad.square().sum(), z)
         with pytest.raises(RuntimeError, match="once"):
             grad.square().sum().backward()
+
+
+# ------------------------------------------------ operators without a backward
+
+def norm_inputs():
+    x, r = (torch.randn(5, 256, device="cuda").to(torch.bfloat16) for _ in range(2))
+    return [x, r, (1 + 0.1 * torch.randn(256, device="cuda")).to(torch.bfloat16)]
+
+
+def int4_inputs():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randint(-2 ** 31, 2 ** 31, (32, 64), generator=g, device="cuda").to(torch.int32)
+    return [torch.randn(5, 256, device="cuda").to(torch.bfloat16),
+            torch.rand(8, 64, device="cuda").to(torch.bfloat16),
+            torch.randn(64, device="cuda").to(torch.bfloat16)], w
+
+
+def bare(ops, F):
+    def int4(f, t, w):
+        return f(t[0], w, t[1], None, t[2])
+    return {
+        "norm": (norm_inputs, lambda t: ops.add_rms_norm(t[0], t[2], t[1])[:2]),
+        "norm fp8": (norm_inputs, lambda t: ops.add_rms_norm(t[0], t[2], t[1], quant=True)),
+        "norm only fp8": (norm_inputs, lambda t: ops.add_rms_norm(t[0], t[2], t[1], quant=True,
+                                                                  normed=False)),
+        "norm out": (norm_inputs, lambda t: ops.add_rms_norm(
+            t[0], t[2], t[1], residual_out=torch.empty(7, 256, device="cuda",
+                                                       dtype=torch.bfloat16)[1:6])),
+        "op norm": (norm_inputs, lambda t: F.add_rms_norm(t[0], t[1], t[2])),
+        "op norm fp8": (norm_inputs, lambda t: F.add_rms_norm_fp8(t[0], t[1], t[2])),
+        "int4": (int4_inputs, lambda t, w: ops.int4_linear(t[0], w, t[1], bias=t[2])),
+        "int4 out": (int4_inputs, lambda t, w: ops.int4_linear(
+            t[0], w, t[1], bias=t[2], out=torch.empty(5, 64, device="cuda", dtype=torch.bfloat16))),
+        "op int4": (int4_inputs, lambda t, w: F.int4_linear(t[0], w, t[1], None, t[2])),
+    }
+
+
+FORMS = ["norm", "norm fp8", "norm only fp8", "norm out", "op norm", "op norm fp8", "int4",
+         "int4 out", "op int4"]
+
+
+def flat(out):
+    return [t for t in (out if isinstance(out, (list, tuple)) else [out]) if t is not None]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_gradient_that_would_be_lost_raises(ops, F, form, which):
+    make, call = bare(ops, F)[form]
+    made = make()
+    inputs, more = made if isinstance(made, tuple) else (made, None)
+    run = (lambda t: call(t)) if more is None else (lambda t: call(t, more))
+    want = flat(run(inputs))
+    assert not any(t.requires_grad for t in want)
+    inputs[which] = inputs[which].requires_grad_(True)
+    got = flat(run(inputs))                                # the forward pass runs as ever
+    assert len(got) == len(want)
+    for a, b in zip(got, want):
+        assert torch.equal(a.detach().view(torch.uint8), b.view(torch.uint8))
+    for out in got:
+        with pytest.raises(RuntimeError, match="no backward"):     # another path does not hide it
+            (out.float().sum() + inputs[which].float().sum()).backward()
+        inputs[which].grad = None
+    with torch.no_grad():
+        assert not any(t.requires_grad for t in flat(run(inputs)))
+
+
+def test_a_written_output_keeps_its_identity(ops):
+    x, r, w = norm_inputs()
+    w.requires_grad_(True)
+    out = ops.add_rms_norm(x, w, r, residual_out=r)
+    assert out[1] is r and r.requires_grad
+    big = torch.zeros(9, 256, device="cuda", dtype=torch.bfloat16)
+    x, r, _ = norm_inputs()
+    out = ops.add_rms_norm(x, w, r, residual_out=big[2:7])
+    assert out[1].data_ptr() == big[2:7].data_ptr()
+    with pytest.raises(RuntimeError, match="no backward"):
+        big.float().sum().backward()
+
+
+def test_the_whole_layer(ops):
+    from test_gpu_moe_block import weights
+    E, H, I, topk = 8, 256, 128, 2
+    norm, gate, w13, s13, w2, s2 = weights(E, H, I, 4)
+    x, r = (torch.randn(6, H, device="cuda").to(torch.bfloat16) for _ in range(2))
+    rest = (w13, s13, w2, s2, topk)
+    want = ops.fp8_moe_block(x, r, norm, gate, *rest)
+    for which in range(4):
+        args = [t.clone() for t in (x, r, norm, gate)]
+        args[which].requires_grad_(True)
+        got = ops.fp8_moe_block(*args, *rest)
+        for a, b in zip(got, want):
+            assert torch.equal(a.detach(), b)
+        for out in (got[0], got[1], got[3]):
+            with pytest.raises(RuntimeError, match="no backward"):
+                (out.float().sum() + args[which].float().sum()).backward()
+    x.requires_grad_(True)
+    out, res, _, logits = ops.fp8_moe_block(x, None, norm, gate, *rest)
+    assert res is x
+    with pytest.raises(RuntimeError, match="no backward"):
+        out.float().sum().backward()

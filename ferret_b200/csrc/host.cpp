@@ -110,6 +110,18 @@ long long row_stride(const at::Tensor& t, const char* name) {
     return T > 1 ? t.stride(0) : K;
 }
 
+// A tensor that the caller passed in to be written: what an operation in place of torch's
+// checks, and (written) the new version that autograd sees of it.
+void writable(const at::Tensor& t, const char* name) {
+    if (at::GradMode::is_enabled() && t.requires_grad() &&
+        (t.is_leaf() || (t.is_view() && t._base().is_leaf())))
+        fail(PyExc_RuntimeError, "%s is a leaf that requires a gradient (or a view of one) and cannot "
+                                 "be written in place", name);
+}
+void written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor make(std::initializer_list<int64_t> shape, at::ScalarType dtype, const at::Tensor& ref) {
     for (int64_t n : shape)
         if (n < 0) fail(PyExc_ValueError, "negative size");
@@ -213,6 +225,7 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         rp = r.data_ptr();
         residual_out = none(a[7]) ? make({T, K}, x.scalar_type(), x) : tensor(a[7], "residual_out");
         like(residual_out, "residual_out", x, x.scalar_type(), {T, K});
+        if (!none(a[7])) writable(residual_out, "residual_out");
     } else if (!none(a[7])) {
         fail(PyExc_ValueError, "residual_out needs a residual");
     }
@@ -230,6 +243,7 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
                               quant ? s.data_ptr<float>() : nullptr,
                               truth(a[5]) ? FERRET_UE8M0_SCALES : 0, on.stream),
           "ferret_add_rms_norm");
+    if (!none(a[7])) written(residual_out);
     return no_backward("ops.add_rms_norm", tuple({y, residual_out, q, s}), a[7],
                        {a[0], a[1], a[2], a[7]});
     END_HANDLE_TH_ERRORS
@@ -360,10 +374,12 @@ PyObject* int4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* bp = like(a[4], "bias", x, x.scalar_type(), {N});
     at::Tensor out = none(a[5]) ? make({T, N}, x.scalar_type(), x) : tensor(a[5], "out");
     void* op = like(out, "out", x, x.scalar_type(), {T, N});
+    if (!none(a[5])) writable(out, "out");
     On on(x);
     check(ferret_int4_linear(x.data_ptr(), ldx, (const int32_t*)wp, sp, (const int32_t*)zp, bp, dt,
                              (int)T, (int)K, (int)N, (int)(K / groups), op, on.stream),
           "ferret_int4_linear");
+    if (!none(a[5])) written(out);
     return no_backward("ops.int4_linear", wrap(out), a[5], {a[0], a[2], a[4], a[5]});
     END_HANDLE_TH_ERRORS
 }

@@ -145,3 +145,57 @@ def test_the_whole_layer(ops):
     assert res is x
     with pytest.raises(RuntimeError, match="no backward"):
         out.float().sum().backward()
+
+
+# ----------------------------------------------------- tensors written in place
+
+def written_calls(ops):
+    x, r, w = norm_inputs()
+    (a, scale, bias), q = int4_inputs()
+    return {
+        "residual_out": (5, 256, lambda out: ops.add_rms_norm(x, w, r, residual_out=out)),
+        "residual": (5, 256, lambda out: ops.add_rms_norm(x, w, out, residual_out=out)),
+        "x": (5, 256, lambda out: ops.add_rms_norm(out, w, r, residual_out=out)),
+        "out": (5, 64, lambda out: ops.int4_linear(a, q, scale, bias=bias, out=out)),
+    }
+
+
+WRITTEN = ["residual_out", "residual", "x", "out"]
+
+
+@pytest.mark.parametrize("what", WRITTEN)
+def test_autograd_sees_that_a_tensor_was_written(ops, what):
+    rows, cols, call = written_calls(ops)[what]
+    leaf = torch.randn(rows, cols, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    for inside in (torch.no_grad(), torch.enable_grad()):
+        h = leaf * 1
+        later = (h * h).sum()                              # saves h
+        before = h._version
+        with inside:
+            call(h)
+        assert h._version > before
+        with pytest.raises(RuntimeError, match="inplace"):
+            later.backward()
+    plain = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+    before = plain._version
+    call(plain)
+    assert plain._version > before
+
+
+@pytest.mark.parametrize("what", WRITTEN)
+def test_leaves_are_not_written_while_autograd_records(ops, what):
+    rows, cols, call = written_calls(ops)[what]
+    leaf = torch.randn(rows, cols, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    big = torch.randn(rows + 2, cols, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    for t, whole in ((leaf, leaf), (big[1:-1], big)):
+        before = whole.detach().clone()
+        with pytest.raises(RuntimeError, match="leaf"):
+            call(t)
+        assert torch.equal(whole.detach(), before)
+    with torch.no_grad():
+        call(leaf)                                         # as an optimizer's step would
+        call(big[1:-1])
+    with torch.inference_mode():
+        inner = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
+        call(inner)
+    call(inner)

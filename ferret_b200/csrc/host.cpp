@@ -110,6 +110,19 @@ long long row_stride(const at::Tensor& t, const char* name) {
     return T > 1 ? t.stride(0) : K;
 }
 
+// Whether `out`, contiguous, shares bytes with the rows of `in` (1-D or 2-D, contiguous rows).
+bool overlap(const at::Tensor& out, const at::Tensor& in) {
+    if (out.numel() == 0 || in.numel() == 0) return false;
+    auto at = [](const at::Tensor& t) { return (int64_t) reinterpret_cast<uintptr_t>(t.data_ptr()); };
+    const int64_t lo = at(out), hi = lo + (int64_t)out.nbytes();
+    const int64_t size = (int64_t)in.element_size(), first = at(in);
+    const int64_t rows = in.dim() == 2 ? in.size(0) : 1, len = in.size(in.dim() - 1) * size;
+    if (rows == 1) return first < hi && first + len > lo;
+    const int64_t step = in.stride(0) * size;              // at least len
+    const int64_t i = first + len > lo ? 0 : (lo - first - len) / step + 1;   // ends behind lo
+    return i < rows && first + i * step < hi;
+}
+
 // A tensor that the caller passed in to be written: what an operation in place of torch's
 // checks, and (written) the new version that autograd sees of it.
 void writable(const at::Tensor& t, const char* name) {
@@ -225,7 +238,17 @@ PyObject* add_rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         rp = r.data_ptr();
         residual_out = none(a[7]) ? make({T, K}, x.scalar_type(), x) : tensor(a[7], "residual_out");
         like(residual_out, "residual_out", x, x.scalar_type(), {T, K});
-        if (!none(a[7])) writable(residual_out, "residual_out");
+        if (!none(a[7])) {
+            // a row is read before it is written: the same rows may be one memory, no others
+            auto same = [&](const at::Tensor& t, long long ld) {
+                return t.data_ptr() == residual_out.data_ptr() && ld == K;
+            };
+            if ((overlap(residual_out, x) && !same(x, ldx)) ||
+                (overlap(residual_out, r) && !same(r, ldr)) || overlap(residual_out, weight))
+                fail(PyExc_ValueError, "residual_out may be x or residual; it must not overlap an "
+                                       "input in another way");
+            writable(residual_out, "residual_out");
+        }
     } else if (!none(a[7])) {
         fail(PyExc_ValueError, "residual_out needs a residual");
     }
@@ -374,7 +397,12 @@ PyObject* int4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* bp = like(a[4], "bias", x, x.scalar_type(), {N});
     at::Tensor out = none(a[5]) ? make({T, N}, x.scalar_type(), x) : tensor(a[5], "out");
     void* op = like(out, "out", x, x.scalar_type(), {T, N});
-    if (!none(a[5])) writable(out, "out");
+    if (!none(a[5])) {
+        for (PyObject* o : {a[0], a[1], a[2], a[3], a[4]})
+            if (!none(o) && overlap(out, THPVariable_Unpack(o)))
+                fail(PyExc_ValueError, "out must not overlap an input");
+        writable(out, "out");
+    }
     On on(x);
     check(ferret_int4_linear(x.data_ptr(), ldx, (const int32_t*)wp, sp, (const int32_t*)zp, bp, dt,
                              (int)T, (int)K, (int)N, (int)(K / groups), op, on.stream),

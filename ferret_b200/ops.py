@@ -451,7 +451,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor |
     residual_out, q, scale): y None with ``normed=False``, residual_out (the
     rounded s) None without a residual, q and scale None without ``quant``.
     Pass ``residual_out`` to have it written there; it may be ``residual`` or
-    ``x`` itself.  With ``quant`` K must be a multiple of 128; K <= 32768.  No
+    ``x`` itself, and must not overlap an input in another way.  With ``quant`` K must be a multiple of 128; K <= 32768.  No
     backward pass."""
     return host().add_rms_norm(x, weight, residual, eps, quant, use_ue8m0, normed, residual_out)
 
@@ -522,7 +522,7 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
     word; 8 without) and bias [N] -> [T, N] of x's type.
 
     g is a multiple of 32, N of 8; x's rows may be strided (by a multiple of 8
-    elements).  Scales are applied in fp32 to the groups' fp32 sums.  Every 32
+    elements).  ``out`` must not overlap an input.  Scales are applied in fp32 to the groups' fp32 sums.  Every 32
     tokens read the weights once: the decode form; large batches go through
     ``moe_wna16_w13`` or a dequantized GEMM.  No backward pass."""
     return host().int4_linear(x, w, w_scale, w_zero, bias, out)

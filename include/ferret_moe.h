@@ -446,7 +446,8 @@ FERRET_API int ferret_moe_balance_loss_backward(const float* grad_loss, const vo
  * along N per word, low nibble first; bias NULL or `dtype` [N]; y `dtype`
  * [T, N] contiguous.  fp32 sums, scales applied in fp32, one rounding at the
  * end; the order of the sums is fixed.  Each pass over the weights serves up
- * to 32 tokens, so more tokens read them again.
+ * to 32 tokens, so more tokens read them again.  y must not overlap an input (CTAs
+ * store columns of a row while others read it).
  * Limits: group % 32 == 0, K % group == 0, K <= 2^20, N % 8 == 0, N < 2^23,
  * T < 2^21, ldx % 8 == 0; x, w and w_scale 16-byte aligned.
  */

@@ -199,3 +199,38 @@ def test_leaves_are_not_written_while_autograd_records(ops, what):
         inner = torch.zeros(rows, cols, device="cuda", dtype=torch.bfloat16)
         call(inner)
     call(inner)
+
+
+def test_written_tensors_that_overlap_inputs_are_refused(ops):
+    """Only refusals here, and neighbours without a shared byte."""
+    K = 128
+    buf = torch.randn(64 * K, device="cuda").to(torch.bfloat16)
+    w = torch.ones(K, device="cuda", dtype=torch.bfloat16)
+    r = torch.randn(4, K, device="cuda").to(torch.bfloat16)
+    rows = lambda at, n=4, step=K: buf.as_strided((n, K), (step, 1), at)
+    x = rows(0)
+    for out in (rows(8), rows(K), rows(3 * K), rows(4 * K - 1)):
+        for first, second in ((x, r), (r, x)):
+            with pytest.raises(ValueError, match="overlap"):
+                ops.add_rms_norm(first, w, second, residual_out=out)
+    with pytest.raises(ValueError, match="overlap"):       # the same start, other rows
+        ops.add_rms_norm(rows(0, step=2 * K), w, r, residual_out=x)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.add_rms_norm(r, buf[K:2 * K], r.clone(), residual_out=x)
+    with pytest.raises(ValueError, match="overlap"):       # between two rows, one byte too far
+        ops.add_rms_norm(rows(0, step=5 * K), w, r, residual_out=rows(K + 1))
+    for first, out in ((rows(0, step=5 * K), rows(K)), (x, x), (x, rows(4 * K))):
+        want = ops.add_rms_norm(first.clone(), w, r)
+        got = ops.add_rms_norm(first, w, r, residual_out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    q = torch.zeros(K // 8, K, dtype=torch.int32, device="cuda")
+    scale = torch.ones(4, K, device="cuda", dtype=torch.bfloat16)
+    x = rows(0)
+    half = lambda t: t.view(torch.bfloat16).flatten()[:4 * K].view(4, K)
+    for kw, out in ((dict(x=x, w=q, w_scale=scale), x), (dict(x=x, w=q, w_scale=scale), rows(8)),
+                    (dict(x=r, w=q, w_scale=scale), half(q)),
+                    (dict(x=r, w=q, w_scale=scale), scale),
+                    (dict(x=r, w=q, w_scale=scale, bias=buf[:K]), x)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.int4_linear(**kw, out=out)
+    assert ops.int4_linear(x, q, scale, out=rows(4 * K)).shape == (4, K)

@@ -377,8 +377,10 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : VPL <= 16 ? 4
                     b2 = max(min(b1, c1), max(b2, c2));
                     b1 = max(b1, c1);
                 }
+                // half the sum of two keys: biases near the largest finite value may not
+                // overflow it
                 float sc = value_of(b1);
-                if (a.group_top == 2 && b2) sc += value_of(b2);
+                if (a.group_top == 2) sc = 0.5f * sc + (b2 ? 0.5f * value_of(b2) : 0.0f);
                 // Distinct images: the lower group first among equals.  A group
                 // is open if fewer than topk_group come before it.
                 const int group = lane >> a.lpg_log;
@@ -393,13 +395,14 @@ __global__ void __launch_bounds__(kRouteWarps * 32, VPL <= 8 ? 6 : VPL <= 16 ? 4
                     for (int k = 0; k < VPL; ++k) list[k] = 0u;
                 // the border between open and closed groups: two sums of two keys,
                 // rounded, with log2(n_group) bits of up to twice the size given away
+                // (or half of all this)
                 const unsigned lo = __reduce_min_sync(kFull, open ? score : 0xffffffffu);
                 const unsigned hi = __reduce_max_sync(kFull, open ? 0u : score);
                 if (hi > last) {
                     const float vl = value_of(lo), vh = value_of(hi);
                     const float big = a.bare ? fmaxf(fabsf(vl), fabsf(vh)) : size;
-                    near = vl - vh <=
-                           2.0f * abs_off + (2.0f * rel + (2 * a.n_group + 6) * 0x1p-23f) * big;
+                    near = vl - vh <= (a.group_top == 2 ? 0.5f : 1.0f) *
+                           (2.0f * abs_off + (2.0f * rel + (2 * a.n_group + 6) * 0x1p-23f) * big);
                 }
             }
             unsigned mine = 0u, more = 0u;        // slot lane's key; the first key not chosen

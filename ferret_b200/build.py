@@ -6,15 +6,19 @@ Each ``csrc/*.cu`` is compiled by nvcc into ``_build/`` (in parallel) and the
 objects are linked into one shared library with the CUDA runtime linked
 statically, so the library loads on machines without a GPU driver (the
 driver-API entry point the TMA descriptors need is resolved at run time
-through the runtime).  ``csrc/host.cpp`` becomes the extension module
-``ferret_b200/_host.so`` (g++ against the installed torch, linked to that
-library next to it).  ``kernel_result.cu`` becomes the benchmark binary
+through the runtime).  ``kernel_result.cu`` becomes the benchmark binary
 ``ferret_b200/ferret_kernel_result`` linked against that library.
+``csrc/host.cpp`` becomes the extension module ``ferret_b200/_host.so`` (g++
+against the installed torch, linked to that library next to it), and again
+when torch or Python changes; without a CUDA torch, g++ or Python's headers it is
+left out, and the library and the C ABI are complete without it.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -27,6 +31,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libferret_moe.so")
 BIN = os.path.join(HERE, "ferret_kernel_result")
 HOST = os.path.join(HERE, "_host.so")
+HOST_FOR = os.path.join(HERE, "_host.for")      # what HOST was built against
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -45,10 +50,13 @@ def _sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cu"))
 
 
+def _headers():
+    return [os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)]
+
+
 def _deps():
-    return [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [
-        os.path.join(INCLUDE, f) for f in os.listdir(INCLUDE)] + [
-        os.path.join(HERE, "kernel_result.cu")]
+    return [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f != "host.cpp"] + _headers() + [
+        os.path.join(HERE, "kernel_result.cu"), __file__]
 
 
 def _stale(target, deps):
@@ -58,12 +66,57 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def host_unavailable() -> str | None:
+    """Why the extension module cannot be built here, or None."""
+    torch = importlib.util.find_spec("torch")
+    if torch is None:
+        return "torch is not installed"
+    if not os.path.exists(os.path.join(os.path.dirname(torch.origin), "lib", "libc10_cuda.so")):
+        return "the installed torch has no CUDA"
+    if not shutil.which("g++"):
+        return "g++ was not found"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers are not installed"
+    return None
+
+
+def _host_for() -> str:
+    try:
+        torch_version = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        import torch
+        torch_version = torch.__version__
+    return f"torch {torch_version}, {sys.implementation.cache_tag}"
+
+
+def _host_stale() -> bool:
+    if _stale(HOST, [os.path.join(CSRC, "host.cpp"), *_headers(), __file__]):
+        return True
+    try:
+        with open(HOST_FOR) as f:
+            return f.read() != _host_for()
+    except OSError:
+        return True
+
+
 def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     srcs = _sources()
-    deps = _deps()
-    if not force and not any(_stale(t, deps + [__file__]) for t in (LIB, BIN, HOST)):
-        return LIB
+    missing = host_unavailable()
+    library = force or any(_stale(t, _deps()) for t in (LIB, BIN))
+    if library:
+        build_library(srcs, verbose, ptxas_verbose)
+    if missing is None:
+        if force or _host_stale():
+            build_host(verbose)
+    elif library:
+        print(f"ferret_b200: extension module not built ({missing}); the library is complete",
+              file=sys.stderr)
+    return LIB
+
+
+def build_library(srcs, verbose: bool = False, ptxas_verbose: bool = False) -> None:
+    """The shared library from its sources, and the benchmark binary."""
     cc = nvcc()
     extra = ["-Xptxas", "-v"] if ptxas_verbose else []
 
@@ -93,8 +146,6 @@ def build(verbose: bool = False, force: bool = False, ptxas_verbose: bool = Fals
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
     build_kernel_result(cc, verbose)
-    build_host(verbose)
-    return LIB
 
 
 def build_kernel_result(cc: str, verbose: bool = False) -> str:
@@ -132,6 +183,8 @@ def build_host(verbose: bool = False) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"host module build failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST)
+    with open(HOST_FOR, "w") as f:
+        f.write(_host_for())
     return HOST
 
 

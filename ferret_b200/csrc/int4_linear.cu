@@ -33,7 +33,9 @@
 // flight thus cost no registers, and few copies carry them: one bulk copy per
 // 512-byte word row left the copy unit at half the HBM rate.  Two CTAs per SM: with
 // three, 72 registers a thread made the compiler compute fragments and scales again
-// (158 warp instructions per 32 x 32 block for 16 tokens against 130).  The eight lanes of
+// (158 warp instructions per 32 x 32 block for 16 tokens against 130).  Two leave 96 (18
+// warps put five on one sub-partition), in which the kernels for 9 to 16 tokens spill 4
+// to 28 bytes a thread, those for more tokens 24 to 72.  The eight lanes of
 // a 16-byte shared-memory read phase hold r = 2q, 2q + 1 and all c; with r
 // standing for 16-byte piece (token) q or q + 4, the swizzle spreads them over
 // all banks.

@@ -26,8 +26,8 @@
 //
 // B200, 32768 x 256 fp32, loss and gradient: 30.7 us (floor 10.4; forward with its join
 // 17.8, backward 12.0 apart), with sigmoids 31.8, with every row below -87 46.  The
-// exponentials and the row sums bound the two large kernels (issue slots 65 and 70 %
-// busy, DRAM under 30 %); four resident CTAs per SM, one wave of each.
+// exponentials and the row sums bound the two large kernels (issue slots 64 % busy in
+// both, DRAM under 30 %); four resident CTAs per SM, one wave of each.
 #include <algorithm>
 #include <type_traits>
 

@@ -523,8 +523,9 @@ def int4_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, *,
 
     g is a multiple of 32, N of 8; x's rows may be strided (by a multiple of 8
     elements).  ``out`` must not overlap an input.  Scales are applied in fp32 to the groups' fp32 sums.  Every 32
-    tokens read the weights once: the decode form; large batches go through
-    ``moe_wna16_w13`` or a dequantized GEMM.  No backward pass."""
+    tokens read the weights once: the decode form.  Larger batches go through a
+    GEMM on dequantized weights, or (bf16, groups of 32, neither zero points nor
+    bias) through ``moe_wna16_w13`` as one expert.  No backward pass."""
     return host().int4_linear(x, w, w_scale, w_zero, bias, out)
 
 

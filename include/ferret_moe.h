@@ -349,8 +349,11 @@ FERRET_API int ferret_int4_moe_w13(const void* hidden_bf16, const void* w_blob,
  * residual_out too; q_scale is [T, K/128].  residual_out may be the same
  * memory as x or residual when that one is contiguous; any other overlap of
  * inputs and outputs is undefined.
- * Limits: K <= 32768; K % 128 == 0 with q_fp8; eps >= 0.  Rows that do not all
- * start on a 16-byte boundary take element-wise loads (same result).
+ * Limits: K <= 32768; K % 128 == 0 with q_fp8; eps >= 0.  mean(s^2) is formed in
+ * fp32 (elements of s below 1e17 in magnitude keep it finite).  Its terms are
+ * added in an order that depends on T, K and the rows' alignment: the same row in
+ * another batch, or at another address, can differ in the last bit of fp32, and
+ * an output by a step where it lies on a rounding border.
  */
 FERRET_API int ferret_add_rms_norm(const void* x, long long ldx, const void* residual,
                                    long long ldr, const void* weight, int weight_dtype, int dtype,
@@ -369,7 +372,10 @@ FERRET_API int ferret_add_rms_norm(const void* x, long long ldx, const void* res
  * group_top (1 or 2) largest keys, and experts outside the topk_group best
  * groups are closed.  The topk largest keys win, in descending order; equal
  * keys (and equal groups) go to the lower index.  The order is that of the
- * exact keys: keys closer than their fp32 rounding are compared in fp64.
+ * exact keys: keys (and group sums) closer than their fp32 rounding are compared
+ * in fp64, so that only what agrees to 53 bits can be taken for equal.
+ * Weights are formed in fp32 (relative error about 1e-7), and so are the
+ * gradients of the next entry point.
  * ids int32 [T, topk]; weights f32 [T, topk] = scale * score (without the
  * bias), divided by the sum of the token's chosen scores with
  * FERRET_ROUTE_RENORM (also where the scores themselves underflow).
@@ -412,6 +418,9 @@ FERRET_API int ferret_moe_route_backward(const float* grad_weights, const void* 
  * probabilities that add up to 1.  logits `dtype` [T, E] with row stride ld,
  * topk_ids int32 [T, topk]; loss, n_tokens one element each.
  * The sums have a fixed order: same inputs on the same device, same bits.
+ * Probabilities and their sums are fp32: a sum is within about 1e-7 of itself
+ * (32768 tokens), a probability d below the row's largest in the exponent (e^-d)
+ * within (10 + 2.25 d) 2^-24 and the roundings of the row's sum.
  * workspace: ferret_moe_balance_loss_workspace_size(T, E) bytes, 16-byte
  * aligned, not shared by calls that can run at the same time.
  * Limits: E <= 1024.
@@ -448,8 +457,8 @@ FERRET_API int ferret_moe_balance_loss_backward(const float* grad_loss, const vo
  * end; the order of the sums is fixed.  Each pass over the weights serves up
  * to 32 tokens, so more tokens read them again.  y must not overlap an input (CTAs
  * store columns of a row while others read it).
- * Limits: group % 32 == 0, K % group == 0, K <= 2^20, N % 8 == 0, N < 2^23,
- * T < 2^21, ldx % 8 == 0; x, w and w_scale 16-byte aligned.
+ * Limits: group % 32 == 0, K % group == 0, K <= 2^20, N % 8 == 0, N <= 65535 * 128,
+ * T <= 65535 * 32, ldx % 8 == 0; x, w and w_scale 16-byte aligned.
  */
 FERRET_API int ferret_int4_linear(const void* x, long long ldx, const int32_t* w,
                                   const void* w_scale, const int32_t* w_zero, const void* bias,

@@ -69,7 +69,7 @@ def _stale(target, deps):
 def host_unavailable() -> str | None:
     """Why the extension module cannot be built here, or None."""
     torch = importlib.util.find_spec("torch")
-    if torch is None:
+    if torch is None or torch.origin is None:
         return "torch is not installed"
     if not os.path.exists(os.path.join(os.path.dirname(torch.origin), "lib", "libc10_cuda.so")):
         return "the installed torch has no CUDA"

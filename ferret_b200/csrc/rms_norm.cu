@@ -20,8 +20,8 @@
 // rows: a persistent grid whose CTAs copy their next rows into a shared-memory
 // ring with bulk copies while they work on the current one; between a row's
 // loads and its stores lies a reduction, and without the ring the memory idles
-// there.  B200, 32768 x 7168 bf16 with all outputs, on several boxes: 357-378 us, 5.6-5.9
-// TB/s (0.86-0.91 of the measured copy rate), against 574 us without the ring; one row 6 us
+// there.  B200, 32768 x 7168 bf16 with all outputs, on several boxes: 353-378 us, 5.6-6.0
+// TB/s (0.86-0.92 of the measured copy rate), against 574 us without the ring; one row 6 us
 // with the host's share, 1021 x 1001 fp16 5.1-5.9 us (10 us element by element).
 //
 // The sum of the squares is an fp32 sum: rows whose elements stay below 1e17 keep it finite.

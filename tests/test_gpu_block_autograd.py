@@ -46,6 +46,26 @@ def test_second_derivatives_raise(F, op, outer):
             grad.square().sum().backward()
 
 
+@pytest.mark.parametrize("op", [route, balance])
+def test_a_captured_backward_pass_is_refused(F, op):
+    """Of a forward pass recorded before the capture on the same stream; the process and
+    the leaf go on."""
+    z = torch.randn(6, 8, device="cuda", requires_grad=True)
+    want, = torch.autograd.grad(op(F, z).sum(), z)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = op(F, z)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="_backward instead"):
+        with torch.cuda.graph(graph, stream=side):
+            torch.autograd.grad(out.sum(), z)
+    torch.cuda.synchronize()
+    again, = torch.autograd.grad(op(F, z).sum(), z)
+    assert torch.equal(again, want)
+
+
 # ------------------------------------------------ operators without a backward
 
 def norm_inputs():

@@ -580,7 +580,7 @@ def fp8_moe_block(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: t
                     ("W2", W2), ("W2_scale", W2_scale)):
         if t.device != x.device:
             raise ValueError(f"{name} must be on the device of x")
-    tied = (x, residual, norm_weight, gate_weight)
+    tied = (x, residual, norm_weight, gate_weight, W13, W13_scale, W2, W2_scale)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tied):
         with torch.no_grad():
             out, res, ids, logits = fp8_moe_block(x, residual, norm_weight, gate_weight, W13,

@@ -160,6 +160,11 @@ def test_the_whole_layer(ops):
         for out in (got[0], got[1], got[3]):
             with pytest.raises(RuntimeError, match="no backward"):
                 (out.float().sum() + args[which].float().sum()).backward()
+    for which in (1, 3):                                   # the scales of the experts' weights
+        moved = list(rest)
+        moved[which] = moved[which].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.fp8_moe_block(x, r, norm, gate, *moved)[0].float().sum().backward()
     x.requires_grad_(True)
     out, res, _, logits = ops.fp8_moe_block(x, None, norm, gate, *rest)
     assert res is x
